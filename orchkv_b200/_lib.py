@@ -109,7 +109,51 @@ class KvBlock(C.Structure):
     ]
 
 
+class Pages(C.Structure):
+    """orchkv_pages_t (include/orchkv/paged_ops.h)."""
+    _fields_ = [("k", vp), ("v", vp), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("n_pages", u32), ("page_tokens", u32),
+                ("n_kv_heads", u32), ("d_head", u32), ("dtype", i32)]
+
+
+class Batch(C.Structure):
+    """orchkv_batch_t."""
+    _fields_ = [("table", vp), ("table_seq_stride", C.c_int64), ("table_head_stride", C.c_int64),
+                ("table_width", u32), ("n_seqs", u32), ("lens", vp), ("starts", vp),
+                ("n_rows", u32), ("max_new", u32)]
+
+
+class Rows(C.Structure):
+    """orchkv_rows_t."""
+    _fields_ = [("p", vp), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class AppendArgs(C.Structure):
+    """orchkv_append_args_t."""
+    _fields_ = [("q", Rows), ("q_out", Rows), ("k", Rows), ("v", Rows), ("n_q_heads", u32),
+                ("rot_dim", u32), ("interleaved", i32), ("scale", f32), ("turns", vp),
+                ("positions", vp), ("positions_64", i32), ("q_norm", vp), ("k_norm", vp),
+                ("eps", f32)]
+
+
+class AttendArgs(C.Structure):
+    """orchkv_attend_args_t."""
+    _fields_ = [("q", Rows), ("out", Rows), ("lse", vp), ("n_q_heads", u32), ("scale", f32),
+                ("window", u32)]
+
+
+class MassArgs(C.Structure):
+    """orchkv_mass_args_t."""
+    _fields_ = [("q", Rows), ("lse", vp), ("mass", vp), ("n_q_heads", u32), ("scale", f32),
+                ("window", u32)]
+
+
 _SIGS = {
+    # operators over paged caches
+    "orchkv_paged_append": (i32, [P(Pages), P(Batch), P(AppendArgs), vp]),
+    "orchkv_paged_attend_workspace": (C.c_size_t, [P(Pages), P(Batch), P(AttendArgs)]),
+    "orchkv_paged_attend": (i32, [P(Pages), P(Batch), P(AttendArgs), vp, C.c_size_t, vp]),
+    "orchkv_paged_block_mass": (i32, [P(Pages), P(Batch), P(MassArgs), vp]),
     # data plane
     "orchkv_init": (i32, [P(OrchkvConfig)]),
     "orchkv_init_ext": (i32, [P(OrchkvConfig), P(OrchkvConfigExt)]),

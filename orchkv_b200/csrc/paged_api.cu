@@ -1,0 +1,189 @@
+// paged_api.cu — the paged operators' C entries: argument checks, the choice
+// of kernels, workspace layout.
+#include "kernels.h"
+#include "paged.cuh"
+
+using namespace okv;
+
+namespace {
+
+constexpr uint32_t kMaxHeadDim = 256;
+constexpr uint64_t kMaxTokens = 1ull << 30;      // of one sequence's table
+
+bool aligned(const void *p, int64_t s0, int64_t s1, size_t e)
+{
+    return p && (uintptr_t)p % 16 == 0 && (s0 * (int64_t)e) % 16 == 0 && (s1 * (int64_t)e) % 16 == 0;
+}
+
+bool rows_ok(const orchkv_rows_t &r, size_t e) { return aligned(r.p, r.row_stride, r.head_stride, e); }
+
+bool shapes_ok(const orchkv_pages_t *p, const orchkv_batch_t *b, bool need_v)
+{
+    if (!p || !b) return false;
+    if (p->dtype != DTYPE_FP16 && p->dtype != DTYPE_BF16 && p->dtype != DTYPE_FP32) return false;
+    const size_t e = dtype_size((DataType)p->dtype);
+    if (p->d_head == 0 || p->d_head > kMaxHeadDim || p->d_head * e % 16) return false;
+    if (p->page_tokens == 0 || p->n_kv_heads == 0 || p->n_kv_heads > 65535 || p->n_pages == 0 ||
+        p->n_pages > 0x7FFFFFFFu)
+        return false;
+    if (!aligned(p->k, p->page_stride, p->head_stride, e) || (p->token_stride * (int64_t)e) % 16)
+        return false;
+    if (need_v && !aligned(p->v, 0, 0, e)) return false;
+    if (b->n_seqs && (!b->table || !b->lens || !b->starts)) return false;
+    if (b->table_width == 0) return false;
+    if ((uint64_t)b->table_width * p->page_tokens > kMaxTokens) return false;
+    if (b->n_seqs > 0x7FFFFFFEu || b->n_rows > 0x7FFFFFFFu) return false;
+    return true;
+}
+
+bool heads_ok(const orchkv_pages_t *p, const orchkv_batch_t *b, uint32_t hq)
+{
+    return hq != 0 && hq % p->n_kv_heads == 0 && (uint64_t)hq * b->n_rows < 0x7FFFFFFFull;
+}
+
+PagesDev pages_dev(const orchkv_pages_t *p)
+{
+    const long long e = (long long)dtype_size((DataType)p->dtype);
+    PagesDev d;
+    d.k = (char *)p->k;
+    d.v = (char *)p->v;
+    d.page_b = p->page_stride * e;
+    d.head_b = p->head_stride * e;
+    d.tok_b = p->token_stride * e;
+    d.n_pages = p->n_pages;
+    d.H = p->n_kv_heads;
+    d.D = p->d_head;
+    d.bs = fast_div(p->page_tokens);
+    return d;
+}
+
+BatchDev batch_dev(const orchkv_batch_t *b)
+{
+    BatchDev d;
+    d.table = b->table;
+    d.ts_seq = b->table_seq_stride;
+    d.ts_head = b->table_head_stride;
+    d.width = b->table_width;
+    d.n = b->n_seqs;
+    d.rows = b->n_rows;
+    d.lens = b->lens;
+    d.starts = b->starts;
+    return d;
+}
+
+RowsDev rows_dev(const orchkv_rows_t &r, size_t e)
+{
+    return RowsDev{(char *)r.p, r.row_stride * (long long)e, r.head_stride * (long long)e};
+}
+
+// What one attend call launches, from what the host knows of it.
+struct AttendPlan {
+    SplitDev simt;
+    size_t bytes;
+};
+
+AttendPlan plan_attend(const orchkv_pages_t *p, const orchkv_batch_t *b, uint32_t hq)
+{
+    AttendPlan pl = {};
+    const uint64_t G = hq / p->n_kv_heads;
+    const uint64_t keys = (uint64_t)b->table_width * p->page_tokens;
+    const uint64_t units = p->n_kv_heads * (b->n_rows * G / kSimtRows + b->n_seqs);
+    pl.simt.ctas = attend_simt_ctas(units * ((keys + kSimtKeys - 1) / kSimtKeys));
+    pl.bytes = (size_t)2 * pl.simt.ctas * kSimtRows * (p->d_head + 2) * sizeof(float);
+    pl.bytes = (pl.bytes + 255) & ~size_t(255);
+    return pl;
+}
+
+}  // namespace
+
+extern "C" {
+
+int orchkv_paged_append(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
+                        const orchkv_append_args_t *args, void *stream)
+{
+    OKV_RANGE("orchkv_paged_append");
+    if (!args || !shapes_ok(pages, batch, true)) return ORCHKV_ERR_INVALID;
+    const size_t e = dtype_size((DataType)pages->dtype);
+    if (args->rot_dim % 2 || args->rot_dim > pages->d_head) return ORCHKV_ERR_INVALID;
+    if (args->rot_dim && !args->turns) return ORCHKV_ERR_INVALID;
+    if (batch->n_rows == 0 || batch->n_seqs == 0) return ORCHKV_OK;
+    if (!rows_ok(args->k, e) || !rows_ok(args->v, e)) return ORCHKV_ERR_INVALID;
+    if (args->n_q_heads && (!rows_ok(args->q, e) || !rows_ok(args->q_out, e))) return ORCHKV_ERR_INVALID;
+    if (args->n_q_heads > 65535 ||
+        (uint64_t)batch->n_rows * (args->n_q_heads + 2ull * pages->n_kv_heads) > 0x7FFFFFFFull)
+        return ORCHKV_ERR_INVALID;
+    AppendDev a;
+    a.q = rows_dev(args->q, e);
+    a.q_out = rows_dev(args->q_out, e);
+    a.k = rows_dev(args->k, e);
+    a.v = rows_dev(args->v, e);
+    a.Hq = args->n_q_heads;
+    a.rot = args->rot_dim;
+    a.inter = args->interleaved != 0;
+    a.pos64 = args->positions_64 != 0;
+    a.scale = args->scale;
+    a.eps = args->eps;
+    a.turns = args->turns;
+    a.pos = args->positions;
+    a.q_norm = args->q_norm;
+    a.k_norm = args->k_norm;
+    return launch_paged_append(pages->dtype, pages_dev(pages), batch_dev(batch), a,
+                               (cudaStream_t)stream);
+}
+
+size_t orchkv_paged_attend_workspace(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
+                                     const orchkv_attend_args_t *args)
+{
+    if (!args || !shapes_ok(pages, batch, false) || !heads_ok(pages, batch, args->n_q_heads)) return 0;
+    if (batch->n_rows == 0 || batch->n_seqs == 0) return 0;
+    return plan_attend(pages, batch, args->n_q_heads).bytes;
+}
+
+int orchkv_paged_attend(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
+                        const orchkv_attend_args_t *args, void *workspace, size_t bytes, void *stream)
+{
+    OKV_RANGE("orchkv_paged_attend");
+    if (!args || !shapes_ok(pages, batch, true) || !heads_ok(pages, batch, args->n_q_heads))
+        return ORCHKV_ERR_INVALID;
+    if (batch->n_rows == 0 || batch->n_seqs == 0) return ORCHKV_OK;
+    const size_t e = dtype_size((DataType)pages->dtype);
+    if (!rows_ok(args->q, e) || !rows_ok(args->out, e)) return ORCHKV_ERR_INVALID;
+    AttendPlan pl = plan_attend(pages, batch, args->n_q_heads);
+    if (!workspace || (uintptr_t)workspace % 256 || bytes < pl.bytes) return ORCHKV_ERR_INVALID;
+    AttendDev a;
+    a.q = rows_dev(args->q, e);
+    a.out = rows_dev(args->out, e);
+    a.lse = args->lse;
+    a.Hq = args->n_q_heads;
+    a.G = args->n_q_heads / pages->n_kv_heads;
+    a.window = args->window;
+    a.sl2 = args->scale * 1.4426950408889634f;
+    const PagesDev p = pages_dev(pages);
+    const BatchDev b = batch_dev(batch);
+    pl.simt.ws = (float *)workspace;
+    return launch_attend_simt(pages->dtype, p, b, a, ClassDev{0, 0xFFFFFFFFu}, pl.simt,
+                              (cudaStream_t)stream);
+}
+
+int orchkv_paged_block_mass(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
+                            const orchkv_mass_args_t *args, void *stream)
+{
+    OKV_RANGE("orchkv_paged_block_mass");
+    if (!args || !shapes_ok(pages, batch, false) || !heads_ok(pages, batch, args->n_q_heads))
+        return ORCHKV_ERR_INVALID;
+    if (batch->n_seqs == 0) return ORCHKV_OK;
+    const size_t e = dtype_size((DataType)pages->dtype);
+    if (!args->mass || (batch->n_rows && (!rows_ok(args->q, e) || !args->lse))) return ORCHKV_ERR_INVALID;
+    MassDev a;
+    a.q = rows_dev(args->q, e);
+    a.lse = args->lse;
+    a.mass = args->mass;
+    a.Hq = args->n_q_heads;
+    a.G = args->n_q_heads / pages->n_kv_heads;
+    a.window = args->window;
+    a.sl2 = args->scale * 1.4426950408889634f;
+    return launch_mass_simt(pages->dtype, pages_dev(pages), batch_dev(batch), a,
+                            ClassDev{0, 0xFFFFFFFFu}, (cudaStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,319 @@
+// paged_split.cuh — how the attention kernels divide a call among their CTAs,
+// and how pieces of one row tile are joined.
+//
+// The work is a list of units (sequence, KV head, tile of R packed rows), each
+// over a range of key tiles (KT keys).  Lengths differ from sequence to
+// sequence and are known on the device alone, so a fixed number of CTAs cut
+// the list into equal shares: every unit gets a weight proportional to the
+// keys it reads (closed form: keys grow by R/G a row tile under the causal
+// mask), CTA c takes [c, c+1) of C equal parts of the sum, and a boundary that
+// falls inside a unit is mapped to a key tile of it.  A unit cut by boundaries
+// leaves one partial (running maximum, sum, unnormalised output) a piece, at
+// most two a CTA, and join_kernel adds the pieces in key order: no atomics,
+// the same result for the same lengths every time.
+#pragma once
+
+#include "paged.cuh"
+
+namespace okv {
+
+typedef unsigned long long ull;
+
+struct Geo {                     // what the division depends on besides the lengths
+    uint32_t R, KT, G, H, window;
+    uint32_t min_rows, max_rows;
+};
+
+__device__ __forceinline__ uint32_t row_tiles(const Geo &g, const SeqDev &s)
+{
+    const uint32_t rows = (uint32_t)s.m * g.G;
+    return rows > g.min_rows && rows <= g.max_rows ? (rows + g.R - 1) / g.R : 0;
+}
+
+// Weight of row tile rt: base + slope * rt, in keys * G; 64 keys' worth stand
+// for a unit's fixed cost.
+__device__ __forceinline__ void weights(const Geo &g, const SeqDev &s, ull *base, ull *slope)
+{
+    const uint32_t c0 = s.c0 > 0 ? s.c0 : 0;
+    if (g.window && g.window < c0 + s.m) {
+        *base = (ull)g.G * (g.window + 64) + g.R;
+        *slope = 0;
+    } else {
+        *base = (ull)g.G * (c0 + 64) + g.R;
+        *slope = g.R;
+    }
+}
+__device__ __forceinline__ ull weight_before(ull base, ull slope, ull rt)
+{
+    return rt * base + slope * (rt * (rt - 1) / 2 * (rt > 0));
+}
+
+// Key tiles [first, first + nt) of row tile rt; nt >= 1 (an empty row tile
+// still has its rows to write).
+__device__ __forceinline__ void key_tiles(const Geo &g, const SeqDev &s, uint32_t rt,
+                                          uint32_t *first, uint32_t *nt)
+{
+    const uint32_t rows = (uint32_t)s.m * g.G;
+    const uint32_t last_row = min((rt + 1) * g.R, rows) - 1;
+    const int hi = min(s.len, s.c0 + (int)(last_row / g.G) + 1);
+    int lo = 0;
+    if (g.window) lo = max(0, s.c0 + (int)(rt * g.R / g.G) - (int)g.window + 1);
+    *first = (uint32_t)lo / g.KT;
+    *nt = hi > lo ? ((uint32_t)hi + g.KT - 1) / g.KT - *first : 1;
+}
+
+struct Pos {
+    uint32_t i, h, rt, t;        // t counts from the unit's first key tile; i == n: the end
+};
+
+// Position of offset x inside sequence i's weight.
+__device__ __forceinline__ Pos inside(const Geo &g, const SeqDev &s, uint32_t i, ull x)
+{
+    ull base, slope;
+    weights(g, s, &base, &slope);
+    const uint32_t RT = row_tiles(g, s);
+    const ull U = weight_before(base, slope, RT);
+    Pos p;
+    p.i = i;
+    p.h = (uint32_t)(x / U);
+    const ull y = x - (ull)p.h * U;
+    ull rt;
+    if (slope == 0) {
+        rt = y / base;
+    } else {
+        const double bb = (double)base - 0.5 * (double)slope;
+        rt = (ull)((sqrt(bb * bb + 2.0 * (double)slope * (double)y) - bb) / (double)slope);
+        if (rt >= RT) rt = RT - 1;
+        while (rt > 0 && weight_before(base, slope, rt) > y) rt--;
+        while (rt + 1 < RT && weight_before(base, slope, rt + 1) <= y) rt++;
+    }
+    p.rt = (uint32_t)rt;
+    uint32_t first, nt;
+    key_tiles(g, s, p.rt, &first, &nt);
+    const ull z = y - weight_before(base, slope, rt), w = base + slope * rt;
+    p.t = (uint32_t)(z * nt / w);
+    return p;
+}
+
+struct SplitShared {
+    ull red[33];
+    ull total;
+    uint32_t seq[2];
+    ull off[2];
+    uint32_t end_seq;
+};
+
+__device__ __forceinline__ ull seq_weight(const Geo &g, const BatchDev &b, uint32_t bs, uint32_t i)
+{
+    if (i >= b.n) return 0;
+    const SeqDev s = load_seq(b, bs, i);
+    const uint32_t RT = row_tiles(g, s);
+    if (RT == 0) return 0;
+    ull base, slope;
+    weights(g, s, &base, &slope);
+    return g.H * weight_before(base, slope, RT);
+}
+
+// Inclusive sum over the block (NT threads) of v; *total the whole sum.
+template <int NT> __device__ __forceinline__ ull block_scan(ull v, ull *red, ull *total)
+{
+    const uint32_t lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const ull u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+        if (lane >= o) v += u;
+    }
+    if (lane == 31) red[wid] = v;
+    __syncthreads();
+    ull before = 0, all = 0;
+#pragma unroll
+    for (int k = 0; k < NT / 32; k++) {
+        if (k < (int)wid) before += red[k];
+        all += red[k];
+    }
+    *total = all;
+    __syncthreads();
+    return before + v;
+}
+
+// Boundaries c and c + 1 of C equal shares, by the whole block; *total 0: no
+// work.  The end of the list is {n, 0, 0, 0}.
+template <int NT>
+__device__ void find_share(const Geo &g, const BatchDev &b, uint32_t bs, uint32_t c, uint32_t C,
+                           SplitShared *sh, Pos *from, Pos *to, ull *W)
+{
+    ull sum = 0, one = 0;
+    for (uint32_t i = threadIdx.x; i < b.n; i += NT) {
+        one = seq_weight(g, b, bs, i);
+        sum += one;
+    }
+    ull total;
+    const ull inc0 = block_scan<NT>(sum, sh->red, &total);
+    *W = total;
+    if (total == 0) return;
+    // shares of ceil(total / C): the last ones may be empty
+    const ull share = (total + C - 1) / C;
+    const ull x[2] = {min(c * share, total), min((c + 1) * share, total)};
+    if (threadIdx.x == 0) sh->seq[0] = sh->seq[1] = b.n;
+    __syncthreads();
+    ull carry = 0;
+    for (uint32_t i0 = 0; i0 < b.n; i0 += NT) {
+        const uint32_t i = i0 + threadIdx.x;
+        ull w, inc, all;
+        if (b.n <= NT) {
+            w = one;
+            inc = inc0;
+            all = total;
+        } else {
+            w = seq_weight(g, b, bs, i);
+            inc = block_scan<NT>(w, sh->red, &all);
+        }
+        const ull ex = carry + inc - w;
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+            if (x[k] >= ex && x[k] < ex + w) {
+                sh->seq[k] = i;
+                sh->off[k] = x[k] - ex;
+            }
+        carry += all;
+        if (carry > x[1]) break;
+    }
+    __syncthreads();
+    Pos *out[2] = {from, to};
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint32_t i = sh->seq[k];
+        if (i >= b.n) *out[k] = Pos{b.n, 0, 0, 0};
+        else *out[k] = inside(g, load_seq(b, bs, i), i, sh->off[k]);
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ bool same_unit(const Pos &a, const Pos &b)
+{
+    return a.i == b.i && a.h == b.h && a.rt == b.rt;
+}
+
+// A row of a unit.
+struct RowInfo {
+    int row;                     // row of the call's tensors, -1 behind the unit's last
+    uint32_t head;               // query head
+    int hi, lo;                  // it attends to tokens lo <= t <= hi
+};
+__device__ __forceinline__ RowInfo row_info(const Geo &g, const SeqDev &s, uint32_t h, uint32_t pr)
+{
+    RowInfo r;
+    if (pr >= (uint32_t)s.m * g.G) {
+        r.row = -1;
+        r.head = 0;
+        r.hi = -1;
+        r.lo = 0;
+        return r;
+    }
+    const uint32_t j = pr / g.G;
+    r.row = s.start + (int)j;
+    r.head = h * g.G + (pr - j * g.G);
+    r.hi = min(s.c0 + (int)j, s.len - 1);
+    r.lo = g.window ? max(0, s.c0 + (int)j - (int)g.window + 1) : 0;
+    return r;
+}
+
+// A partial slot: m[R], l[R], then acc[R][D].
+__device__ __forceinline__ float *slot_of(float *ws, uint32_t slot, uint32_t R, uint32_t D)
+{
+    return ws + (size_t)slot * R * (D + 2);
+}
+__host__ __device__ inline size_t slot_floats(uint32_t R, uint32_t D) { return (size_t)R * (D + 2); }
+
+// The pieces of every cut unit into its rows.  Block c looks at boundary c: it
+// works if that is the first boundary inside a unit.  Pieces lie in slot
+// 2c'+1 (the unit's start, held by CTA c' = c - 1) and in slots 2c, 2c+2, ...
+template <class T, int NT>
+__global__ void __launch_bounds__(NT)
+join_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp)
+{
+    cudaGridDependencySynchronize();
+    __shared__ SplitShared sh;
+    const uint32_t c = blockIdx.x + 1;
+    Pos prev, at;
+    ull W;
+    find_share<NT>(g, b, p.bs.d, c - 1, sp.ctas, &sh, &prev, &at, &W);
+    if (W == 0 || at.i >= b.n || at.t == 0) return;
+    if (same_unit(prev, at) && prev.t > 0) return;
+    const SeqDev s = load_seq(b, p.bs.d, at.i);
+    uint32_t first, nt;
+    key_tiles(g, s, at.rt, &first, &nt);
+    // the boundaries after c that fall into the unit, as offsets of the sequence
+    const ull share = (W + sp.ctas - 1) / sp.ctas;
+    __shared__ uint32_t slots[1024];
+    __shared__ uint32_t n_slots;
+    if (threadIdx.x == 0) {
+        uint32_t k = 0;
+        slots[k++] = 2 * (c - 1) + 1;
+        ull off = sh.off[1];
+        Pos cur = at;
+        ull base, slope;
+        weights(g, s, &base, &slope);
+        const ull seqW = g.H * weight_before(base, slope, row_tiles(g, s));
+        for (uint32_t cc = c; cc < sp.ctas; cc++) {
+            off += share;
+            Pos nx = off < seqW && cc + 1 < sp.ctas ? inside(g, s, at.i, off) : Pos{b.n, 0, 0, 0};
+            const bool in = same_unit(nx, at);
+            if ((in ? nx.t : nt) > cur.t && k < 1024) slots[k++] = 2 * cc;
+            if (!in) break;
+            cur = nx;
+        }
+        n_slots = k;
+    }
+    __syncthreads();
+    const uint32_t K = n_slots, D = p.D, R = g.R;
+    const uint32_t d4 = D / 4;
+    for (uint32_t e = threadIdx.x; e < R * d4; e += NT) {
+        const uint32_t rr = e / d4, d = (e - rr * d4) * 4;
+        const RowInfo ri = row_info(g, s, at.h, at.rt * R + rr);
+        if (ri.row < 0) continue;
+        float M = -INFINITY;
+        for (uint32_t k = 0; k < K; k++) M = fmaxf(M, slot_of(sp.ws, slots[k], R, D)[rr]);
+        const float Ms = M == -INFINITY ? 0.f : M;
+        float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t k = 0; k < K; k++) {
+            const float *sl = slot_of(sp.ws, slots[k], R, D);
+            const float w = exp2f(sl[rr] - Ms);
+            L += w * sl[R + rr];
+            const float4 v = *(const float4 *)(sl + 2 * R + (size_t)rr * D + d);
+            // a piece without an attended token holds zeros
+            o[0] += w * v.x;
+            o[1] += w * v.y;
+            o[2] += w * v.z;
+            o[3] += w * v.w;
+        }
+        const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+        T *dst = (T *)(a.out.p + (long long)ri.row * a.out.row_b + (long long)ri.head * a.out.head_b) + d;
+#pragma unroll
+        for (int j = 0; j < 4; j++) dst[j] = from_f<T>(o[j] * inv);
+        if (a.lse && d == 0)
+            a.lse[(size_t)ri.row * a.Hq + ri.head] =
+                L > 0.f ? (Ms + log2f(L)) * 0.69314718055994531f : L == 0.f ? -INFINITY : L;
+    }
+}
+
+// A launch that may begin before the one in front of it in the stream has
+// ended (the kernel waits itself with cudaGridDependencySynchronize).
+template <class... P, class... A>
+cudaError_t launch_after(void (*k)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t s,
+                         A... args)
+{
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(grid);
+    c.blockDim = dim3(block);
+    c.dynamicSmemBytes = smem;
+    c.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, k, args...);
+}
+
+}  // namespace okv
