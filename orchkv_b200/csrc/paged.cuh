@@ -209,10 +209,17 @@ struct SplitDev {
     float *ws;
 };
 constexpr uint32_t kSimtRows = 8, kSimtKeys = 128;
-uint32_t attend_simt_ctas(unsigned long long tiles);
-int launch_attend_simt(int dtype, const PagesDev &p, const BatchDev &b, const AttendDev &a,
+uint32_t attend_simt_ctas(unsigned long long units, unsigned long long keys);
+int launch_attend_simt(const PagesDev &p, const BatchDev &b, const AttendDev &a,
                        const ClassDev &cl, const SplitDev &sp, cudaStream_t s);
-int launch_mass_simt(int dtype, const PagesDev &p, const BatchDev &b, const MassDev &a,
+int launch_mass_simt(const PagesDev &p, const BatchDev &b, const MassDev &a,
+                     const ClassDev &cl, cudaStream_t s);
+
+constexpr uint32_t kRowsRows = 16;
+uint32_t attend_rows_ctas(uint32_t D, unsigned long long units, unsigned long long keys);
+int launch_attend_rows(int dtype, const PagesDev &p, const BatchDev &b, const AttendDev &a,
+                       const ClassDev &cl, const SplitDev &sp, cudaStream_t s);
+int launch_mass_rows(int dtype, const PagesDev &p, const BatchDev &b, const MassDev &a,
                      const ClassDev &cl, cudaStream_t s);
 
 }  // namespace okv

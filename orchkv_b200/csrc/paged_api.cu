@@ -78,7 +78,7 @@ RowsDev rows_dev(const orchkv_rows_t &r, size_t e)
 
 // What one attend call launches, from what the host knows of it.
 struct AttendPlan {
-    SplitDev simt;
+    SplitDev rows;           // the kernel for few rows a sequence (fp32: the CUDA-core one)
     size_t bytes;
 };
 
@@ -87,9 +87,11 @@ AttendPlan plan_attend(const orchkv_pages_t *p, const orchkv_batch_t *b, uint32_
     AttendPlan pl = {};
     const uint64_t G = hq / p->n_kv_heads;
     const uint64_t keys = (uint64_t)b->table_width * p->page_tokens;
-    const uint64_t units = p->n_kv_heads * (b->n_rows * G / kSimtRows + b->n_seqs);
-    pl.simt.ctas = attend_simt_ctas(units * ((keys + kSimtKeys - 1) / kSimtKeys));
-    pl.bytes = (size_t)2 * pl.simt.ctas * kSimtRows * (p->d_head + 2) * sizeof(float);
+    const uint32_t R = p->dtype == DTYPE_FP32 ? kSimtRows : kRowsRows;
+    const uint64_t units = p->n_kv_heads * (b->n_rows * G / R + b->n_seqs);
+    pl.rows.ctas = p->dtype == DTYPE_FP32 ? attend_simt_ctas(units, keys)
+                                          : attend_rows_ctas(p->d_head, units, keys);
+    pl.bytes = (size_t)2 * pl.rows.ctas * R * (p->d_head + 2) * sizeof(float);
     pl.bytes = (pl.bytes + 255) & ~size_t(255);
     return pl;
 }
@@ -160,9 +162,10 @@ int orchkv_paged_attend(const orchkv_pages_t *pages, const orchkv_batch_t *batch
     a.sl2 = args->scale * 1.4426950408889634f;
     const PagesDev p = pages_dev(pages);
     const BatchDev b = batch_dev(batch);
-    pl.simt.ws = (float *)workspace;
-    return launch_attend_simt(pages->dtype, p, b, a, ClassDev{0, 0xFFFFFFFFu}, pl.simt,
-                              (cudaStream_t)stream);
+    const ClassDev all = {0, 0xFFFFFFFFu};
+    pl.rows.ws = (float *)workspace;
+    if (pages->dtype == DTYPE_FP32) return launch_attend_simt(p, b, a, all, pl.rows, (cudaStream_t)stream);
+    return launch_attend_rows(pages->dtype, p, b, a, all, pl.rows, (cudaStream_t)stream);
 }
 
 int orchkv_paged_block_mass(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
@@ -182,8 +185,11 @@ int orchkv_paged_block_mass(const orchkv_pages_t *pages, const orchkv_batch_t *b
     a.G = args->n_q_heads / pages->n_kv_heads;
     a.window = args->window;
     a.sl2 = args->scale * 1.4426950408889634f;
-    return launch_mass_simt(pages->dtype, pages_dev(pages), batch_dev(batch), a,
-                            ClassDev{0, 0xFFFFFFFFu}, (cudaStream_t)stream);
+    const ClassDev all = {0, 0xFFFFFFFFu};
+    const PagesDev p = pages_dev(pages);
+    const BatchDev b = batch_dev(batch);
+    if (pages->dtype == DTYPE_FP32) return launch_mass_simt(p, b, a, all, (cudaStream_t)stream);
+    return launch_mass_rows(pages->dtype, p, b, a, all, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -314,24 +314,21 @@ int mass(const PagesDev &p, const BatchDev &b, const MassDev &a, const ClassDev 
 
 }  // namespace
 
-uint32_t attend_simt_ctas(unsigned long long tiles)
+uint32_t attend_simt_ctas(unsigned long long units, unsigned long long keys)
 {
+    const unsigned long long tiles = units * ((keys + kSimtKeys - 1) / kSimtKeys);
     return (uint32_t)(tiles < 148 * 4 ? tiles : 148 * 4);
 }
 
-int launch_attend_simt(int dtype, const PagesDev &p, const BatchDev &b, const AttendDev &a,
+int launch_attend_simt(const PagesDev &p, const BatchDev &b, const AttendDev &a,
                        const ClassDev &cl, const SplitDev &sp, cudaStream_t s)
 {
-    if (dtype == DTYPE_BF16) return attend<__nv_bfloat16>(p, b, a, cl, sp, s);
-    if (dtype == DTYPE_FP16) return attend<__half>(p, b, a, cl, sp, s);
     return attend<float>(p, b, a, cl, sp, s);
 }
 
-int launch_mass_simt(int dtype, const PagesDev &p, const BatchDev &b, const MassDev &a,
+int launch_mass_simt(const PagesDev &p, const BatchDev &b, const MassDev &a,
                      const ClassDev &cl, cudaStream_t s)
 {
-    if (dtype == DTYPE_BF16) return mass<__nv_bfloat16>(p, b, a, cl, s);
-    if (dtype == DTYPE_FP16) return mass<__half>(p, b, a, cl, s);
     return mass<float>(p, b, a, cl, s);
 }
 

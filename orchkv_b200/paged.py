@@ -173,65 +173,78 @@ class PagedKV:
         self.n_pages, self.page_tokens, self.head_dim, self.dtype = n_pages, tokens, head_dim, dtype
         self.n_kv_heads = heads                   # None: as many as the call's tables have
         self._args = (k_ptr, v_ptr) + strides + (n_pages, tokens)
+        self._align = 16 // dtype.itemsize
         self._by_heads = {}
 
     def _pages(self, heads: int):
-        pg = self._by_heads.get(heads)
-        if pg is None:
-            pg = self._by_heads[heads] = self._C.Pages(*self._args, heads, self.head_dim,
-                                                       _DTYPES[self.dtype])
+        _need(heads > 0, "a table of no heads")
+        pg = self._by_heads[heads] = self._C.Pages(*self._args, heads, self.head_dim,
+                                                   _DTYPES[self.dtype])
         return pg
 
     # -- argument checks -----------------------------------------------------
 
     def _batch(self, table, lens, starts, rows, max_new):
         """(pages handle, KV heads, the batch's arguments)."""
-        i32 = torch.int32
-        slab = self.n_kv_heads is None
-        _need(table.dtype == i32 and lens.dtype == i32 and starts.dtype == i32,
-              "table, lens and starts must be int32")
-        _need(table.dim() == (3 if slab else 2), "table must be [sequences, KV heads, width]" if slab
-              else "table must be [sequences, width]")
-        n = lens.shape[0] if lens.dim() == 1 else -1
-        _need(n == table.shape[0] and starts.dim() == 1 and starts.shape[0] == n + 1,
-              "table, lens and starts must have n, n and n + 1 entries")
-        _need(table.stride(-1) == 1 and lens.is_contiguous() and starts.is_contiguous(),
-              "table rows, lens and starts must be contiguous")
-        _need(table.shape[-1] > 0, "a table of no blocks")
-        dev = self._dev
-        _need(table.get_device() == dev and lens.get_device() == dev and starts.get_device() == dev,
-              "every tensor must be on the pages' device")
+        i32, dev, slab = torch.int32, self._dev, self.n_kv_heads is None
+        shape = table.shape
+        if table.dtype != i32 or lens.dtype != i32 or starts.dtype != i32:
+            raise ValueError("table, lens and starts must be int32")
+        if len(shape) != (3 if slab else 2):
+            raise ValueError("table must be [sequences, KV heads, width]" if slab
+                             else "table must be [sequences, width]")
+        n, width = shape[0], shape[-1]
+        if lens.shape != (n,) or starts.shape != (n + 1,):
+            raise ValueError("table, lens and starts must have n, n and n + 1 entries")
+        st = table.stride()
+        if st[-1] != 1 or not lens.is_contiguous() or not starts.is_contiguous():
+            raise ValueError("table rows, lens and starts must be contiguous")
+        if width == 0:
+            raise ValueError("a table of no blocks")
+        if table.get_device() != dev or lens.get_device() != dev or starts.get_device() != dev:
+            raise ValueError("every tensor must be on the pages' device")
         if max_new is None:
             max_new = rows
-        _need(max_new >= 0, "max_new must not be negative")
-        heads = table.shape[1] if slab else self.n_kv_heads
-        _need(heads > 0, "a table of no heads")
-        return self._pages(heads), heads, (
-            table.data_ptr(), table.stride(0), table.stride(1) if slab else 0, table.shape[-1], n,
-            lens.data_ptr(), starts.data_ptr(), rows, max_new)
+        elif max_new < 0:
+            raise ValueError("max_new must not be negative")
+        heads = shape[1] if slab else self.n_kv_heads
+        pg = self._by_heads.get(heads) or self._pages(heads)
+        return pg, heads, (table.data_ptr(), st[0], st[1] if slab else 0, width, n, lens.data_ptr(),
+                           starts.data_ptr(), rows, max_new)
 
     def _rows(self, x, name, heads=None, rows=None):
         """Checks a row tensor; its (pointer, row stride, head stride)."""
-        _need(x.dim() == 3 and x.shape[2] == self.head_dim and (heads is None or x.shape[1] == heads)
-              and (rows is None or x.shape[0] == rows),
-              f"{name} must be [rows, heads, {self.head_dim}]"
-              + ("" if heads is None else f" with {heads} heads"))
-        _need(x.dtype == self.dtype, f"{name} must be {self.dtype} as the pages are")
-        p, s = x.data_ptr(), x.stride()
-        align = 16 // x.element_size()
-        _need(x.numel() == 0 or (s[2] == 1 and s[0] % align == 0 and s[1] % align == 0 and p % 16 == 0),
-              f"{name}: heads must be contiguous, pointer and strides multiples of 16 bytes")
-        _need(x.get_device() == self._dev, f"{name} must be on the pages' device")
+        shape = x.shape
+        if (len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads)
+                or (rows is not None and shape[0] != rows)):
+            raise ValueError(f"{name} must be [rows, heads, {self.head_dim}]"
+                             + ("" if heads is None else f" with {heads} heads")
+                             + ("" if rows is None else f" and {rows} rows"))
+        if x.dtype != self.dtype:
+            raise ValueError(f"{name} must be {self.dtype} as the pages are")
+        p, s, align = x.data_ptr(), x.stride(), self._align
+        if (s[2] != 1 or s[0] % align or s[1] % align or p % 16) and x.numel():
+            raise ValueError(f"{name}: heads must be contiguous, pointer and strides multiples of "
+                             "16 bytes")
+        if x.get_device() != self._dev:
+            raise ValueError(f"{name} must be on the pages' device")
         if x.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires a gradient, which these operators do not have")
         return p, s[0], s[1]
 
+    def _heads(self, hq, heads, window):
+        if hq == 0 or hq % heads:
+            raise ValueError(f"{hq} query heads do not share {heads} KV heads")
+        if window < 0:
+            raise ValueError("window must not be negative")
+
     def _call(self, fn, *args):
-        if torch.cuda.current_device() == self._dev:
-            rc = fn(*args, torch.cuda.current_stream(self._dev).cuda_stream)
+        dev = self._dev
+        if torch.cuda.current_device() == dev:
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
         else:
-            with torch.cuda.device(self._dev):
-                rc = fn(*args, torch.cuda.current_stream(self._dev).cuda_stream)
+            with torch.cuda.device(dev):
+                rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
         if rc != 0:
             raise RuntimeError(f"orchkv_{fn.__name__} failed: {rc}")
 
@@ -267,9 +280,10 @@ class PagedKV:
         norms = []
         for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
             if w is not None:
-                _need(w.shape == (self.head_dim,) and w.dtype == self.dtype and w.is_contiguous()
-                      and w.get_device() == self._dev,
-                      f"{name} must be [{self.head_dim}] {self.dtype} on the pages' device")
+                if (w.shape != (self.head_dim,) or w.dtype != self.dtype or not w.is_contiguous()
+                        or w.get_device() != self._dev):
+                    raise ValueError(f"{name} must be [{self.head_dim}] {self.dtype}, contiguous, on "
+                                     "the pages' device")
             norms.append(0 if w is None else w.data_ptr())
         rot, inter, scale, turns = 0, 0, 1.0, 0
         if rotary is not None:
@@ -294,8 +308,7 @@ class PagedKV:
         qa = self._rows(q, "q")
         hq = q.shape[1]
         pg, heads, batch = self._batch(table, lens, starts, rows, max_new)
-        _need(hq > 0 and hq % heads == 0, f"{hq} query heads do not share {heads} KV heads")
-        _need(window >= 0, "window must not be negative")
+        self._heads(hq, heads, window)
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         oa = self._rows(out, "out", hq, rows)
@@ -317,16 +330,17 @@ class PagedKV:
         qa = self._rows(q, "q")
         hq = q.shape[1]
         pg, heads, batch = self._batch(table, lens, starts, rows, max_new)
-        _need(hq > 0 and hq % heads == 0, f"{hq} query heads do not share {heads} KV heads")
-        _need(window >= 0, "window must not be negative")
-        _need(lse.dtype == torch.float32 and lse.shape == (rows, hq) and lse.is_contiguous()
-              and lse.get_device() == self._dev, f"lse must be fp32 [{rows}, {hq}], contiguous")
+        self._heads(hq, heads, window)
+        if (lse.dtype != torch.float32 or lse.shape != (rows, hq) or not lse.is_contiguous()
+                or lse.get_device() != self._dev):
+            raise ValueError(f"lse must be fp32 [{rows}, {hq}], contiguous, on the pages' device")
         shape = (lens.shape[0], heads, table.shape[-1])
         if out is None:
             out = torch.empty(shape, dtype=torch.float32, device=q.device)
         else:
-            _need(out.shape == shape and out.dtype == torch.float32 and out.is_contiguous()
-                  and out.get_device() == self._dev, f"out must be fp32 {list(shape)}, contiguous")
+            if (out.shape != shape or out.dtype != torch.float32 or not out.is_contiguous()
+                    or out.get_device() != self._dev):
+                raise ValueError(f"out must be fp32 {list(shape)}, contiguous, on the pages' device")
         args = (hq, self.head_dim ** -0.5 if scale is None else scale, window)
         self._call(self._C.paged_block_mass, pg, batch, qa, lse.data_ptr(), out.data_ptr(), args)
         return out
