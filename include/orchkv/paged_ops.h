@@ -132,6 +132,11 @@ typedef struct orchkv_mass_args {
 int orchkv_paged_block_mass(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
                             const orchkv_mass_args_t *args, void *stream);
 
+/* ORCHKV_ERR_CUDA once a wait inside one of these kernels has run out (2 s;
+ * its call's results are then not complete), ORCHKV_OK otherwise.
+ * Synchronous. */
+int orchkv_paged_status(void);
+
 #ifdef __cplusplus
 }
 #endif

@@ -37,7 +37,7 @@ NVFLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
 CU_SOURCES = ["sched_kernels.cu", "select_kernels.cu", "pool_kernels.cu", "tm.cu",
               "api.cu", "comm.cu", "static_select.cu", "manager_kernels.cu",
               "integrity_kernels.cu", "paged_api.cu", "paged_append.cu", "paged_simt.cu",
-              "paged_rows.cu"]
+              "paged_rows.cu", "paged_tile.cu"]
 
 
 CHECKED = os.path.join(PKG, "_checked")        # the checked build's library and module

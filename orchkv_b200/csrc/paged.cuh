@@ -222,4 +222,11 @@ int launch_attend_rows(int dtype, const PagesDev &p, const BatchDev &b, const At
 int launch_mass_rows(int dtype, const PagesDev &p, const BatchDev &b, const MassDev &a,
                      const ClassDev &cl, cudaStream_t s);
 
+constexpr uint32_t kTileRows = 256;
+// Whether the tile kernel takes these pages (and a call with this scale).
+bool attend_tile_takes(const PagesDev &p, int dtype, float sl2);
+uint32_t attend_tile_ctas(unsigned long long units, unsigned long long keys);
+int launch_attend_tile(int dtype, const PagesDev &p, const BatchDev &b, const AttendDev &a,
+                       const ClassDev &cl, const SplitDev &sp, cudaStream_t s);
+
 }  // namespace okv

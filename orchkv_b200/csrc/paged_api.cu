@@ -1,5 +1,7 @@
 // paged_api.cu — the paged operators' C entries: argument checks, the choice
 // of kernels, workspace layout.
+#include <algorithm>
+
 #include "kernels.h"
 #include "paged.cuh"
 
@@ -76,22 +78,35 @@ RowsDev rows_dev(const orchkv_rows_t &r, size_t e)
     return RowsDev{(char *)r.p, r.row_stride * (long long)e, r.head_stride * (long long)e};
 }
 
+// Sequences with more packed rows than this go to the tile kernel, in calls
+// that may have any.
+constexpr uint32_t kFewRows = 64;
+
 // What one attend call launches, from what the host knows of it.
 struct AttendPlan {
-    SplitDev rows;           // the kernel for few rows a sequence (fp32: the CUDA-core one)
+    SplitDev rows, tile;     // ctas 0: not launched
+    ClassDev few, many;
     size_t bytes;
 };
 
-AttendPlan plan_attend(const orchkv_pages_t *p, const orchkv_batch_t *b, uint32_t hq)
+AttendPlan plan_attend(const orchkv_pages_t *p, const orchkv_batch_t *b, const orchkv_attend_args_t *args)
 {
     AttendPlan pl = {};
-    const uint64_t G = hq / p->n_kv_heads;
+    const uint64_t G = args->n_q_heads / p->n_kv_heads, H = p->n_kv_heads;
     const uint64_t keys = (uint64_t)b->table_width * p->page_tokens;
+    const uint64_t most = (uint64_t)(b->max_new < b->n_rows ? b->max_new : b->n_rows) * G;
+    const bool tile = most > kFewRows && attend_tile_takes(pages_dev(p), p->dtype, args->scale);
     const uint32_t R = p->dtype == DTYPE_FP32 ? kSimtRows : kRowsRows;
-    const uint64_t units = p->n_kv_heads * (b->n_rows * G / R + b->n_seqs);
+    uint64_t units = H * (b->n_rows * G / R + b->n_seqs);
+    if (tile) units = std::min(units, H * b->n_seqs * (kFewRows / R));
+    pl.few = ClassDev{0, tile ? kFewRows : 0xFFFFFFFFu};
+    pl.many = ClassDev{kFewRows, 0xFFFFFFFFu};
     pl.rows.ctas = p->dtype == DTYPE_FP32 ? attend_simt_ctas(units, keys)
                                           : attend_rows_ctas(p->d_head, units, keys);
-    pl.bytes = (size_t)2 * pl.rows.ctas * R * (p->d_head + 2) * sizeof(float);
+    if (tile) pl.tile.ctas = attend_tile_ctas(H * (b->n_rows * G / kTileRows + b->n_seqs), keys);
+    // both may use the same memory: the tile kernel starts when the rows are joined
+    const size_t row = (p->d_head + 2) * sizeof(float) * 2;
+    pl.bytes = std::max(pl.rows.ctas * R, pl.tile.ctas * kTileRows) * row;
     pl.bytes = (pl.bytes + 255) & ~size_t(255);
     return pl;
 }
@@ -138,7 +153,7 @@ size_t orchkv_paged_attend_workspace(const orchkv_pages_t *pages, const orchkv_b
 {
     if (!args || !shapes_ok(pages, batch, false) || !heads_ok(pages, batch, args->n_q_heads)) return 0;
     if (batch->n_rows == 0 || batch->n_seqs == 0) return 0;
-    return plan_attend(pages, batch, args->n_q_heads).bytes;
+    return plan_attend(pages, batch, args).bytes;
 }
 
 int orchkv_paged_attend(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
@@ -150,7 +165,7 @@ int orchkv_paged_attend(const orchkv_pages_t *pages, const orchkv_batch_t *batch
     if (batch->n_rows == 0 || batch->n_seqs == 0) return ORCHKV_OK;
     const size_t e = dtype_size((DataType)pages->dtype);
     if (!rows_ok(args->q, e) || !rows_ok(args->out, e)) return ORCHKV_ERR_INVALID;
-    AttendPlan pl = plan_attend(pages, batch, args->n_q_heads);
+    AttendPlan pl = plan_attend(pages, batch, args);
     if (!workspace || (uintptr_t)workspace % 256 || bytes < pl.bytes) return ORCHKV_ERR_INVALID;
     AttendDev a;
     a.q = rows_dev(args->q, e);
@@ -162,10 +177,12 @@ int orchkv_paged_attend(const orchkv_pages_t *pages, const orchkv_batch_t *batch
     a.sl2 = args->scale * 1.4426950408889634f;
     const PagesDev p = pages_dev(pages);
     const BatchDev b = batch_dev(batch);
-    const ClassDev all = {0, 0xFFFFFFFFu};
-    pl.rows.ws = (float *)workspace;
-    if (pages->dtype == DTYPE_FP32) return launch_attend_simt(p, b, a, all, pl.rows, (cudaStream_t)stream);
-    return launch_attend_rows(pages->dtype, p, b, a, all, pl.rows, (cudaStream_t)stream);
+    pl.rows.ws = pl.tile.ws = (float *)workspace;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (pages->dtype == DTYPE_FP32) return launch_attend_simt(p, b, a, pl.few, pl.rows, st);
+    const int rc = launch_attend_rows(pages->dtype, p, b, a, pl.few, pl.rows, st);
+    if (rc || pl.tile.ctas == 0) return rc;
+    return launch_attend_tile(pages->dtype, p, b, a, pl.many, pl.tile, st);
 }
 
 int orchkv_paged_block_mass(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
