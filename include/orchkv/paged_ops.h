@@ -128,9 +128,12 @@ typedef struct orchkv_mass_args {
  * g and the tokens t of block b of exp(scale * q[r, h] . K[t] - lse[r, h]),
  * the probability orchkv_paged_attend gave t: what tm_report_attn_probs sums
  * out of a stored map.  Blocks that hold no attended token get 0.  Sums run
- * in one fixed order.  pages->v is not read.  Asynchronous. */
+ * in one fixed order.  pages->v is not read.  workspace as for
+ * orchkv_paged_attend (NULL where the size is 0).  Asynchronous. */
+size_t orchkv_paged_block_mass_workspace(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
+                                         const orchkv_mass_args_t *args);
 int orchkv_paged_block_mass(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
-                            const orchkv_mass_args_t *args, void *stream);
+                            const orchkv_mass_args_t *args, void *workspace, size_t bytes, void *stream);
 
 /* ORCHKV_ERR_CUDA once a wait inside one of these kernels has run out (2 s;
  * its call's results are then not complete), ORCHKV_OK otherwise.

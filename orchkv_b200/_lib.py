@@ -154,7 +154,8 @@ _SIGS = {
     "orchkv_paged_attend_workspace": (C.c_size_t, [P(Pages), P(Batch), P(AttendArgs)]),
     "orchkv_paged_attend": (i32, [P(Pages), P(Batch), P(AttendArgs), vp, C.c_size_t, vp]),
     "orchkv_paged_status": (i32, []),
-    "orchkv_paged_block_mass": (i32, [P(Pages), P(Batch), P(MassArgs), vp]),
+    "orchkv_paged_block_mass_workspace": (C.c_size_t, [P(Pages), P(Batch), P(MassArgs)]),
+    "orchkv_paged_block_mass": (i32, [P(Pages), P(Batch), P(MassArgs), vp, C.c_size_t, vp]),
     # data plane
     "orchkv_init": (i32, [P(OrchkvConfig)]),
     "orchkv_init_ext": (i32, [P(OrchkvConfig), P(OrchkvConfigExt)]),

@@ -226,6 +226,11 @@ constexpr uint32_t kTileRows = 256;
 // Whether the tile kernel takes these pages (and a call with this scale).
 bool attend_tile_takes(const PagesDev &p, int dtype, float sl2);
 uint32_t attend_tile_ctas(unsigned long long units, unsigned long long keys);
+bool mass_tile_takes(const PagesDev &p, int dtype, float sl2, const RowsDev &q, uint32_t G);
+uint32_t mass_tile_ctas(unsigned long long units, unsigned long long rows);
+constexpr uint32_t kMassSlot = 32;       // floats of a partial slot
+int launch_mass_tile(int dtype, const PagesDev &p, const BatchDev &b, const MassDev &a,
+                     const ClassDev &cl, const SplitDev &sp, cudaStream_t s);
 int launch_attend_tile(int dtype, const PagesDev &p, const BatchDev &b, const AttendDev &a,
                        const ClassDev &cl, const SplitDev &sp, cudaStream_t s);
 

@@ -111,6 +111,29 @@ AttendPlan plan_attend(const orchkv_pages_t *p, const orchkv_batch_t *b, const o
     return pl;
 }
 
+struct MassPlan {
+    SplitDev tile;           // ctas 0: not launched
+    ClassDev few, many;
+    size_t bytes;
+};
+
+MassPlan plan_mass(const orchkv_pages_t *p, const orchkv_batch_t *b, const orchkv_mass_args_t *args)
+{
+    MassPlan pl = {};
+    const size_t e = dtype_size((DataType)p->dtype);
+    const uint32_t G = args->n_q_heads / p->n_kv_heads;
+    const uint64_t keys = (uint64_t)b->table_width * p->page_tokens;
+    const uint64_t new_rows = b->max_new < b->n_rows ? b->max_new : b->n_rows;
+    const bool tile = new_rows * G > kFewRows &&
+                      mass_tile_takes(pages_dev(p), p->dtype, args->scale, rows_dev(args->q, e), G);
+    pl.few = ClassDev{0, tile ? kFewRows : 0xFFFFFFFFu};
+    pl.many = ClassDev{kFewRows, 0xFFFFFFFFu};
+    if (tile)
+        pl.tile.ctas = mass_tile_ctas((uint64_t)p->n_kv_heads * b->n_seqs * ((keys + 255) / 256), new_rows * G);
+    pl.bytes = ((size_t)2 * pl.tile.ctas * kMassSlot * sizeof(float) + 255) & ~size_t(255);
+    return pl;
+}
+
 }  // namespace
 
 extern "C" {
@@ -185,8 +208,16 @@ int orchkv_paged_attend(const orchkv_pages_t *pages, const orchkv_batch_t *batch
     return launch_attend_tile(pages->dtype, p, b, a, pl.many, pl.tile, st);
 }
 
+size_t orchkv_paged_block_mass_workspace(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
+                                         const orchkv_mass_args_t *args)
+{
+    if (!args || !shapes_ok(pages, batch, false) || !heads_ok(pages, batch, args->n_q_heads)) return 0;
+    if (batch->n_seqs == 0) return 0;
+    return plan_mass(pages, batch, args).bytes;
+}
+
 int orchkv_paged_block_mass(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
-                            const orchkv_mass_args_t *args, void *stream)
+                            const orchkv_mass_args_t *args, void *workspace, size_t bytes, void *stream)
 {
     OKV_RANGE("orchkv_paged_block_mass");
     if (!args || !shapes_ok(pages, batch, false) || !heads_ok(pages, batch, args->n_q_heads))
@@ -194,6 +225,8 @@ int orchkv_paged_block_mass(const orchkv_pages_t *pages, const orchkv_batch_t *b
     if (batch->n_seqs == 0) return ORCHKV_OK;
     const size_t e = dtype_size((DataType)pages->dtype);
     if (!args->mass || (batch->n_rows && (!rows_ok(args->q, e) || !args->lse))) return ORCHKV_ERR_INVALID;
+    MassPlan pl = plan_mass(pages, batch, args);
+    if (pl.bytes && (!workspace || (uintptr_t)workspace % 256 || bytes < pl.bytes)) return ORCHKV_ERR_INVALID;
     MassDev a;
     a.q = rows_dev(args->q, e);
     a.lse = args->lse;
@@ -202,11 +235,14 @@ int orchkv_paged_block_mass(const orchkv_pages_t *pages, const orchkv_batch_t *b
     a.G = args->n_q_heads / pages->n_kv_heads;
     a.window = args->window;
     a.sl2 = args->scale * 1.4426950408889634f;
-    const ClassDev all = {0, 0xFFFFFFFFu};
     const PagesDev p = pages_dev(pages);
     const BatchDev b = batch_dev(batch);
-    if (pages->dtype == DTYPE_FP32) return launch_mass_simt(p, b, a, all, (cudaStream_t)stream);
-    return launch_mass_rows(pages->dtype, p, b, a, all, (cudaStream_t)stream);
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (pages->dtype == DTYPE_FP32) return launch_mass_simt(p, b, a, pl.few, st);
+    const int rc = launch_mass_rows(pages->dtype, p, b, a, pl.few, st);
+    if (rc || pl.tile.ctas == 0) return rc;
+    pl.tile.ws = (float *)workspace;
+    return launch_mass_tile(pages->dtype, p, b, a, pl.many, pl.tile, st);
 }
 
 }  // extern "C"

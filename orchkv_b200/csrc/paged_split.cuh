@@ -137,14 +137,15 @@ template <int NT> __device__ __forceinline__ ull block_scan(ull v, ull *red, ull
 }
 
 // Boundaries c and c + 1 of C equal shares, by the whole block; *total 0: no
-// work.  The end of the list is {n, 0, 0, 0}.
-template <int NT>
-__device__ void find_share(const Geo &g, const BatchDev &b, uint32_t bs, uint32_t c, uint32_t C,
-                           SplitShared *sh, Pos *from, Pos *to, ull *W)
+// work.  The end of the list is {n, 0, 0, 0}.  weight(i) is sequence i's part
+// of the list, where(s, i, x) the position of offset x in it.
+template <int NT, class Weight, class Where>
+__device__ void find_share(const BatchDev &b, uint32_t bs, uint32_t c, uint32_t C, SplitShared *sh, Pos *from,
+                           Pos *to, ull *W, Weight weight, Where where)
 {
     ull sum = 0, one = 0;
     for (uint32_t i = threadIdx.x; i < b.n; i += NT) {
-        one = seq_weight(g, b, bs, i);
+        one = weight(i);
         sum += one;
     }
     ull total;
@@ -165,7 +166,7 @@ __device__ void find_share(const Geo &g, const BatchDev &b, uint32_t bs, uint32_
             inc = inc0;
             all = total;
         } else {
-            w = seq_weight(g, b, bs, i);
+            w = i < b.n ? weight(i) : 0;
             inc = block_scan<NT>(w, sh->red, &all);
         }
         const ull ex = carry + inc - w;
@@ -184,9 +185,16 @@ __device__ void find_share(const Geo &g, const BatchDev &b, uint32_t bs, uint32_
     for (int k = 0; k < 2; k++) {
         const uint32_t i = sh->seq[k];
         if (i >= b.n) *out[k] = Pos{b.n, 0, 0, 0};
-        else *out[k] = inside(g, load_seq(b, bs, i), i, sh->off[k]);
+        else *out[k] = where(load_seq(b, bs, i), i, sh->off[k]);
     }
     __syncthreads();
+}
+template <int NT>
+__device__ void find_share(const Geo &g, const BatchDev &b, uint32_t bs, uint32_t c, uint32_t C,
+                           SplitShared *sh, Pos *from, Pos *to, ull *W)
+{
+    find_share<NT>(b, bs, c, C, sh, from, to, W, [&](uint32_t i) { return seq_weight(g, b, bs, i); },
+                   [&](const SeqDev &s, uint32_t i, ull x) { return inside(g, s, i, x); });
 }
 
 __device__ __forceinline__ bool same_unit(const Pos &a, const Pos &b)

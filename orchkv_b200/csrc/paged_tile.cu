@@ -459,9 +459,535 @@ int go(const CUtensorMap &km, const CUtensorMap &vm, const PagesDev &p, const Ba
     return ORCHKV_OK;
 }
 
+// ---- masses of chunks --------------------------------------------------------------
+//
+// The product is turned round: the 128 keys of a tile are the rows of the
+// accumulator, so a thread owns a key and its sum over all query rows is a sum
+// of its own lane's columns, with no exchange between threads.  Nothing but the
+// sums leaves the CTA: 2 D products a score against one power of two, so the
+// special function unit (16 a clock) would take twice the tensor core's time;
+// half of the powers go to the FMA units as polynomials (ex2_poly).  A unit is
+// 256 keys (one tile a softmax group) against the rows that may attend to
+// them; the K tiles stay, the query rows stream through a ring (by TMA: a box
+// of G heads by 128/G tokens is 128 packed rows), scores alternate between two
+// buffers a group.  CTAs cut the list of units as the attention does; pieces
+// of one unit are added by mass_join_kernel in row order.
+
+constexpr int kMassThreads = 384;
+constexpr uint32_t kMK = 256;                          // keys of a unit
+
+constexpr int kMassRing = 3;                           // query tiles
+
+template <int DP> struct MassCfg {
+    static constexpr uint32_t tile = 128 * DP * 2;
+    static constexpr size_t tiles = (size_t)(4 + kMassRing) * tile;    // two units' keys, the ring
+};
+
+struct MassGeo {
+    uint32_t G, H, window, min_rows, toks;             // toks: tokens of a query tile
+};
+
+// Key tiles of a sequence, and the tokens that may attend to one.
+struct MassSeq {
+    uint32_t kf, kn;                                   // unit k covers keys (kf + k) * 256, k < kn
+};
+__device__ __forceinline__ MassSeq mass_seq(const MassGeo &g, const SeqDev &s)
+{
+    MassSeq q = {0, 0};
+    if ((uint32_t)s.m * g.G <= g.min_rows) return q;
+    const int hi = s.len;
+    int lo = g.window ? s.c0 - (int)g.window + 1 : 0;
+    lo = lo < 0 ? 0 : lo;
+    q.kf = (uint32_t)lo / kMK;
+    const uint32_t kl = ((uint32_t)hi + kMK - 1) / kMK;
+    q.kn = kl > q.kf ? kl - q.kf : 1;                  // one unit at least: it writes the zeros
+    return q;
+}
+// Tokens [a, e) of the sequence's rows that may attend to keys [k0, k0 + 256).
+__device__ __forceinline__ void mass_tokens(const MassGeo &g, const SeqDev &s, uint32_t k0, int *a, int *e)
+{
+    *a = max(0, (int)k0 - s.c0);
+    *e = s.m;
+    if (g.window) *e = min(s.m, (int)k0 + (int)kMK - 1 - s.c0 + (int)g.window);
+    if (*e < *a) *e = *a;
+}
+// Weight of unit k: its tokens and 16 for the unit itself; without a window the
+// tokens fall by 256 a unit from the sequence's first new key on.
+__device__ __forceinline__ ull mass_before(const MassGeo &g, const SeqDev &s, const MassSeq &q, ull k)
+{
+    const ull m = s.m;
+    if (g.window) return k * (min(m, (ull)g.window + kMK) + 16);
+    const ull c0 = s.c0 > 0 ? s.c0 : 0, f = c0 / kMK;  // unit f still has every token
+    ull v = k * (m + 16);
+    if (k > f + 1) {
+        const ull n = k - 1 - f;                       // units f+1 .. k-1
+        v -= kMK * ((f + 1 + k - 1) * n / 2) - c0 * n;
+    }
+    return v;
+}
+__device__ __forceinline__ ull mass_weight(const MassGeo &g, const BatchDev &b, uint32_t bs, uint32_t i)
+{
+    const SeqDev s = load_seq(b, bs, i);
+    const MassSeq q = mass_seq(g, s);
+    return q.kn ? g.H * mass_before(g, s, q, q.kn) : 0;
+}
+// Query tiles of unit k, at least one.
+__device__ __forceinline__ uint32_t mass_tiles(const MassGeo &g, const SeqDev &s, const MassSeq &q, uint32_t k)
+{
+    int a, e;
+    mass_tokens(g, s, (q.kf + k) * kMK, &a, &e);
+    const uint32_t n = ((uint32_t)(e - a) + g.toks - 1) / g.toks;
+    return n ? n : 1;
+}
+__device__ __forceinline__ Pos mass_inside(const MassGeo &g, const SeqDev &s, uint32_t i, ull x)
+{
+    const MassSeq q = mass_seq(g, s);
+    const ull U = mass_before(g, s, q, q.kn);
+    Pos p;
+    p.i = i;
+    p.h = (uint32_t)(x / U);
+    const ull y = x - (ull)p.h * U;
+    uint32_t lo = 0, hi = q.kn;                        // the last k with before(k) <= y
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (mass_before(g, s, q, mid) <= y) lo = mid;
+        else hi = mid;
+    }
+    p.rt = lo;
+    const ull z = y - mass_before(g, s, q, lo), w = mass_before(g, s, q, lo + 1) - mass_before(g, s, q, lo);
+    p.t = (uint32_t)(z * mass_tiles(g, s, q, lo) / w);
+    return p;
+}
+
+struct MassWalk {
+    const MassGeo &g;
+    const BatchDev &b;
+    uint32_t bs;
+    Pos at, end;
+    SeqDev s;
+    MassSeq q;
+    uint32_t nt, t0, t1;
+    int a, e;                                          // tokens of the unit
+    bool stop;
+
+    __device__ bool settle()
+    {
+        while (at.i < b.n) {
+            s = load_seq(b, bs, at.i);
+            q = mass_seq(g, s);
+            if (q.kn == 0) { at = Pos{at.i + 1, 0, 0, 0}; continue; }
+            stop = same_unit(at, end);
+            mass_tokens(g, s, key0(), &a, &e);
+            nt = mass_tiles(g, s, q, at.rt);
+            t0 = at.t;
+            t1 = stop ? end.t : nt;
+            if (t0 < t1) return true;
+            if (stop) return false;
+            advance();
+        }
+        return false;
+    }
+    __device__ uint32_t key0() const { return (q.kf + at.rt) * kMK; }
+    __device__ void advance()
+    {
+        at.t = 0;
+        if (++at.rt == q.kn) {
+            at.rt = 0;
+            if (++at.h == g.H) { at.h = 0; at.i++; }
+        }
+    }
+    __device__ bool next()
+    {
+        if (stop) return false;
+        advance();
+        return settle();
+    }
+};
+
+struct MassShared {
+    ull k_full[2], k_empty[2], q_full[kMassRing], q_empty[kMassRing], s_full[4], s_empty[4], drain, sums[3];
+    uint32_t tmem;
+    int dead;
+    alignas(16) float lse[kMassRing][128];                     // of a query tile's rows, times log2(e)
+    alignas(16) float key[kMK];
+    SplitShared split;
+};
+
+static_assert(MassCfg<128>::tiles + sizeof(MassShared) <= 232448, "over an SM's 227 KB");
+
+// The zeros in front of a sequence's first unit and behind its last.
+__device__ __forceinline__ void mass_zero_rest(const MassWalk &w, const BatchDev &b, const PagesDev &p, float *mass,
+                                               uint32_t tid, uint32_t nt)
+{
+    float *out = mass + ((size_t)w.at.i * w.g.H + w.at.h) * b.width;
+    const uint32_t per = kMK / p.bs.d;
+    if (w.at.rt == 0)
+        for (uint32_t k = tid; k < min(w.q.kf * per, b.width); k += nt) out[k] = 0.f;
+    if (w.at.rt + 1 == w.q.kn)
+        for (uint32_t k = (w.q.kf + w.q.kn) * per + tid; k < b.width; k += nt) out[k] = 0.f;
+}
+
+template <class T, int DP>
+__global__ void __launch_bounds__(kMassThreads, 1)
+mass_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap qmap, MassGeo g,
+                 PagesDev p, BatchDev b, MassDev a, SplitDev sp, int by_head)
+{
+    using Cfg = MassCfg<DP>;
+    constexpr int RQ = kMassRing;
+    constexpr uint32_t halves = DP / 64;
+    // no static part, so the tiles start on the 1024 bytes their swizzle needs
+    extern __shared__ __align__(1024) char raw[];
+    MassShared &sh = *(MassShared *)(raw + Cfg::tiles);
+    const uint32_t base = smem_addr(raw);
+    if (base & 1023) {
+        if (threadIdx.x == 0) g_paged_dead = 1;
+        return;
+    }
+    const uint32_t keys_s = base, ring = base + 4 * Cfg::tile;
+    const uint32_t wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    MassWalk w{g, b, p.bs.d};
+    ull W;
+    find_share<kMassThreads>(b, p.bs.d, blockIdx.x, sp.ctas, &sh.split, &w.at, &w.end, &W,
+                             [&](uint32_t i) { return mass_weight(g, b, p.bs.d, i); },
+                             [&](const SeqDev &s, uint32_t i, ull x) { return mass_inside(g, s, i, x); });
+    cudaTriggerProgrammaticLaunchCompletion();
+    if (W == 0) return;
+    if (!w.settle()) return;
+
+    const uint32_t cols = g.toks * g.G;                    // of a query tile
+    if (threadIdx.x == 0) {
+        for (int k = 0; k < 2; k++) {
+            mbar_init(smem_addr(&sh.k_full[k]), 1);
+            mbar_init(smem_addr(&sh.k_empty[k]), 1);
+        }
+        for (int k = 0; k < RQ; k++) {
+            mbar_init(smem_addr(&sh.q_full[k]), 2);
+            mbar_init(smem_addr(&sh.q_empty[k]), 9);
+        }
+        for (int k = 0; k < 3; k++) mbar_init(smem_addr(&sh.sums[k]), k < 2 ? 4 : 8);
+        for (int k = 0; k < 4; k++) {
+            mbar_init(smem_addr(&sh.s_full[k]), 1);
+            mbar_init(smem_addr(&sh.s_empty[k]), 4);
+        }
+        mbar_init(smem_addr(&sh.drain), 1);
+        sh.dead = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // rows of the query tiles that no box covers: zeros, not stale bits
+    for (uint32_t e = threadIdx.x; e < RQ * (128 - cols) * halves * 8; e += kMassThreads) {
+        const uint32_t c = e & 7, x = (e >> 3) % halves, r = (e >> 3) / halves;
+        const uint32_t st = r / (128 - cols), row = cols + r - st * (128 - cols);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                         ring + st * Cfg::tile + x * 128 * 128 + row * 128 + c * 16), "r"(0) : "memory");
+    }
+    for (uint32_t e = threadIdx.x; e < RQ * 128; e += kMassThreads) sh.lse[e >> 7][e & 127] = 0.f;
+    fence_async();
+    if (wid == 1) tm_alloc(smem_addr(&sh.tmem), 512);
+    tm_before();
+    __syncthreads();
+    tm_after();
+    const uint32_t tm = sh.tmem;
+    volatile int *dead = &sh.dead;
+
+    if (wid < 4) {
+      regs_down<88>();
+      if (wid == 0) {
+        // ---- loads ----
+        const uint32_t bs = p.bs.d, per = bs < 128 ? 128 / bs : 1, box = bs < 128 ? bs : 128;
+        uint32_t u_no = 0, st = 0, ph = 0, issued = 0;
+        bool ok = true;
+        do {
+            const uint32_t kb = u_no & 1, k0 = w.key0();
+            int pg[2];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const uint32_t key = k0 + x * 128 + lane * bs;
+                pg[x] = lane < per && (int)key < w.s.len ? page_of(b, p.n_pages, w.at.i, w.at.h, key / p.bs) : -1;
+            }
+            const uint32_t n = __popc(__ballot_sync(0xFFFFFFFFu, pg[0] >= 0)) +
+                               __popc(__ballot_sync(0xFFFFFFFFu, pg[1] >= 0));
+            ok = mbar_wait(smem_addr(&sh.k_empty[kb]), (u_no >> 1 & 1) ^ 1, dead);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            const uint32_t kbar = smem_addr(&sh.k_full[kb]);
+            if (lane == 0) mbar_expect(kbar, n * box * 128 * halves);
+            __syncwarp();
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+                if (pg[x] >= 0)
+#pragma unroll
+                    for (uint32_t c = 0; c < halves; c++)
+                        tma4(keys_s + (kb * 2 + x) * Cfg::tile + c * 128 * 128 + lane * box * 128, &kmap,
+                             (int)c * 64, bs < 128 ? 0 : (int)((k0 + x * 128) % bs), by_head ? 0 : (int)w.at.h,
+                             pg[x], kbar);
+            u_no++;
+            for (uint32_t t = w.t0; t < w.t1; t++) {
+                ok = mbar_wait(smem_addr(&sh.q_empty[st]), ph ^ 1, dead);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) break;
+                if (lane == 0) {
+                    const uint32_t bar = smem_addr(&sh.q_full[st]);
+                    mbar_expect(bar, cols * 128 * halves);
+                    const int row = w.s.start + w.a + (int)(t * g.toks);
+#pragma unroll
+                    for (uint32_t c = 0; c < halves; c++)
+                        tma3(ring + st * Cfg::tile + c * 128 * 128, &qmap, (int)c * 64, (int)(w.at.h * g.G), row, bar);
+                }
+                __syncwarp();
+                issued++;
+                if (++st == RQ) { st = 0; ph ^= 1; }
+            }
+        } while (ok && w.next());
+        if (!ok) {
+            // leave no copy in flight behind
+            if (lane == 0) {
+                for (uint32_t k = 0; k < (uint32_t)RQ && k < issued; k++) {
+                    st = st == 0 ? RQ - 1 : st - 1;
+                    if (st == RQ - 1) ph ^= 1;
+                    mbar_drain(smem_addr(&sh.q_full[st]), ph);
+                }
+                for (uint32_t k = 0; k < 2 && k < u_no; k++)
+                    mbar_drain(smem_addr(&sh.k_full[(u_no - 1 - k) & 1]), (u_no - 1 - k) >> 1 & 1);
+            }
+            __syncwarp();
+        }
+      } else if (wid == 1) {
+        // ---- products ----
+        if (lane == 0) {
+            const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+            const uint32_t id = inst_desc(f, 128, 128, 0);
+            uint32_t u_no = 0, st = 0, ph = 0, tile = 0;
+            bool ok = true;
+            do {
+                const uint32_t kb = u_no & 1;
+                ok = mbar_wait(smem_addr(&sh.k_full[kb]), u_no >> 1 & 1, dead);
+                for (uint32_t t = w.t0; ok && t < w.t1; t++, tile++) {
+                    ok = mbar_wait(smem_addr(&sh.q_full[st]), ph, dead);
+                    for (int x = 0; ok && x < 2; x++) {
+                        const uint32_t sb = x * 2 + (tile & 1);
+                        ok = mbar_wait(smem_addr(&sh.s_empty[sb]), (tile >> 1 & 1) ^ 1, dead);
+                        if (!ok) break;
+                        tm_after();
+                        const uint32_t ka = keys_s + (kb * 2 + x) * Cfg::tile, qa = ring + st * Cfg::tile;
+#pragma unroll
+                        for (int k = 0; k < DP / 16; k++) {
+                            const uint32_t o = (k >> 2) * 128 * 128 + (k & 3) * 32;
+                            mma_ss(tm + sb * 128, smem_desc(ka + o, 16, 1024), smem_desc(qa + o, 16, 1024), id, k > 0);
+                        }
+                        tm_commit(smem_addr(&sh.s_full[sb]));
+                    }
+                    if (!ok) break;
+                    tm_commit(smem_addr(&sh.q_empty[st]));
+                    if (++st == RQ) { st = 0; ph ^= 1; }
+                }
+                if (ok) tm_commit(smem_addr(&sh.k_empty[kb]));
+                u_no++;
+            } while (ok && w.next());
+            if (!ok) {
+                tm_commit(smem_addr(&sh.drain));
+                mbar_drain(smem_addr(&sh.drain), 0);
+            }
+        }
+        __syncwarp();
+      } else if (wid == 2) {
+        // ---- the rows' lse ----
+        uint32_t st = 0, ph = 0;
+        bool ok = true;
+        do {
+            for (uint32_t t = w.t0; t < w.t1; t++) {
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t c = lane + 32 * k, j = c / g.G;
+                    const int tok = w.a + (int)(t * g.toks + j);
+                    v[k] = c < cols ? 0.f : INFINITY;  // a column of no row weighs nothing
+                    if (c < cols && tok < w.e)
+                        v[k] = a.lse[(size_t)(w.s.start + tok) * a.Hq + w.at.h * g.G + (c - j * g.G)] * kLog2e;
+                }
+                ok = mbar_wait(smem_addr(&sh.q_empty[st]), ph ^ 1, dead);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) break;
+#pragma unroll
+                for (int k = 0; k < 4; k++) sh.lse[st][lane + 32 * k] = v[k];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&sh.q_full[st]));
+                if (++st == RQ) { st = 0; ph ^= 1; }
+            }
+        } while (ok && w.next());
+      }
+    } else {
+        regs_up<208>();
+        // ---- sums of one half's keys ----
+        const int x = (wid - 4) >> 2;
+        const uint32_t r = threadIdx.x - 128 - x * 128;
+        const uint32_t lanes = (wid & 3) << 21;
+        const ull sl2 = f2(a.sl2, a.sl2), neg = f2(-1.f, -1.f);
+        uint32_t st = 0, ph = 0, tile = 0, sum_ph = 0;
+        bool ok = true, live = true;
+        while (live && ok) {
+            const int key = (int)(w.key0() + x * 128 + r);
+            const uint32_t blk = (uint32_t)key / p.bs;
+            const bool there = key < w.s.len && page_of(b, p.n_pages, w.at.i, w.at.h, blk) >= 0;
+            // tokens [ja, je) of the rows attend to this key
+            const int ja = max(0, key - w.s.c0);
+            int je = w.s.m;
+            if (g.window) je = min(je, key - w.s.c0 + (int)g.window);
+            ull sum[2] = {0, 0};
+            for (uint32_t t = w.t0; t < w.t1; t++, tile++) {
+                const uint32_t sb = x * 2 + (tile & 1);
+                ok = mbar_wait(smem_addr(&sh.s_full[sb]), tile >> 1 & 1, dead) &&
+                     mbar_wait(smem_addr(&sh.q_full[st]), ph, dead);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) break;
+                tm_after();
+                const uint32_t S = tm + sb * 128 + lanes;
+                const int j0 = w.a + (int)(t * g.toks);
+                int lo = (ja - j0) * (int)g.G, hi = (min(je, w.e) - j0) * (int)g.G;
+                lo = lo < 0 ? 0 : lo;
+                hi = hi > (int)cols ? (int)cols : hi;
+                if (!there) hi = 0;
+                const bool all = __all_sync(0xFFFFFFFFu, lo == 0 && hi == (int)cols);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    float s[32];
+                    tm_ld32(S + c * 32, s);
+                    tm_wait_ld();
+                    if (c == 3) {                      // the scores are all read
+                        tm_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_addr(&sh.s_empty[sb]));
+                    }
+                    const float4 *ls = (const float4 *)&sh.lse[st][c * 32];
+                    if (all) {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const float4 l4 = ls[j];
+                            const ull u = fma2(f2(s[4 * j], s[4 * j + 1]), sl2, mul2(f2(l4.x, l4.y), neg));
+                            const ull v = fma2(f2(s[4 * j + 2], s[4 * j + 3]), sl2, mul2(f2(l4.z, l4.w), neg));
+                            float e0, e1;
+                            unf2(u, &e0, &e1);
+                            sum[0] = add2(sum[0], f2(ex2(e0), ex2(e1)));
+                            sum[1] = add2(sum[1], ex2_poly<5>(v));
+                        }
+                    } else {
+                        const int l0 = lo - c * 32, h0 = hi - c * 32;
+                        uint32_t bits = h0 <= 0 ? 0u : h0 >= 32 ? 0xFFFFFFFFu : (1u << h0) - 1;
+                        bits &= l0 > 31 ? 0u : l0 <= 0 ? 0xFFFFFFFFu : ~((1u << l0) - 1);
+                        if (__any_sync(0xFFFFFFFFu, bits != 0)) {
+#pragma unroll
+                            for (int j = 0; j < 8; j++) {
+                                const float4 l4 = ls[j];
+                                const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+                                float e[4];
+#pragma unroll
+                                for (int k = 0; k < 4; k++)
+                                    e[k] = bits >> (4 * j + k) & 1 ? ex2(s[4 * j + k] * a.sl2 - lv[k]) : 0.f;
+                                sum[0] = add2(sum[0], f2(e[0], e[1]));
+                                sum[1] = add2(sum[1], f2(e[2], e[3]));
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&sh.q_empty[st]));
+                if (++st == RQ) { st = 0; ph ^= 1; }
+            }
+            if (!ok) break;
+            float s0, s1, s2, s3;
+            unf2(sum[0], &s0, &s1);
+            unf2(sum[1], &s2, &s3);
+            sh.key[x * 128 + r] = (s0 + s1) + (s2 + s3);
+            const bool whole = w.t0 == 0 && w.t1 == w.nt;
+            const uint32_t bs = p.bs.d;
+            // blocks of at most 128 keys belong to one group, larger ones to both
+            const bool both = bs > 128;
+            const uint32_t bar = smem_addr(&sh.sums[both ? 2 : x]);
+            auto meet = [&] {                          // of the threads that add a block's keys
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar);
+                ok = mbar_wait(bar, sum_ph, dead);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                sum_ph ^= 1;
+            };
+            meet();
+            if (!ok) break;
+            const uint32_t nb = both ? 1 : 128 / bs;
+            if (r < nb && !(both && x == 1)) {
+                float y = 0.f;
+                for (uint32_t k = 0; k < bs; k++) y += sh.key[x * 128 + r * bs + k];
+                const uint32_t lb = (both ? 0 : x * nb) + r;          // block of the unit
+                const uint32_t gb = w.key0() / bs + lb;
+                if (!whole) sp.ws[(size_t)(2 * blockIdx.x + (w.t0 == 0 ? 1 : 0)) * kMassSlot + lb] = y;
+                else if (gb < b.width) a.mass[((size_t)w.at.i * g.H + w.at.h) * b.width + gb] = y;
+            }
+            if (w.t0 == 0) mass_zero_rest(w, b, p, a.mass, x * 128 + r, 256);
+            meet();
+            live = w.next();
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && sh.dead) g_paged_dead = 1;
+    if (wid == 1) tm_free(tm, 512);
+}
+
+// Pieces of cut units: slots as join_kernel finds them.
+__global__ void __launch_bounds__(128)
+mass_join_kernel(MassGeo g, PagesDev p, BatchDev b, MassDev a, SplitDev sp)
+{
+    cudaGridDependencySynchronize();
+    __shared__ SplitShared sh;
+    const uint32_t c = blockIdx.x + 1;
+    Pos prev, at;
+    ull W;
+    find_share<128>(b, p.bs.d, c - 1, sp.ctas, &sh, &prev, &at, &W,
+                    [&](uint32_t i) { return mass_weight(g, b, p.bs.d, i); },
+                    [&](const SeqDev &s, uint32_t i, ull x) { return mass_inside(g, s, i, x); });
+    if (W == 0 || at.i >= b.n || at.t == 0) return;
+    if (same_unit(prev, at) && prev.t > 0) return;
+    const SeqDev s = load_seq(b, p.bs.d, at.i);
+    const MassSeq q = mass_seq(g, s);
+    const ull share = (W + sp.ctas - 1) / sp.ctas, seqW = g.H * mass_before(g, s, q, q.kn);
+    const uint32_t nb = kMK / p.bs.d, lb = threadIdx.x;
+    const uint32_t gb = (q.kf + at.rt) * nb + lb, nt = mass_tiles(g, s, q, at.rt);
+    float y = 0.f;
+    if (lb < nb) y = sp.ws[(size_t)(2 * (c - 1) + 1) * kMassSlot + lb];
+    ull off = sh.off[1];
+    Pos cur = at;
+    for (uint32_t cc = c; cc < sp.ctas; cc++) {
+        off += share;
+        const Pos nx = off < seqW && cc + 1 < sp.ctas ? mass_inside(g, s, at.i, off) : Pos{b.n, 0, 0, 0};
+        const bool in = same_unit(nx, at);
+        if ((in ? nx.t : nt) > cur.t && lb < nb) y += sp.ws[(size_t)2 * cc * kMassSlot + lb];
+        if (!in) break;
+        cur = nx;
+    }
+    if (lb < nb && gb < b.width) a.mass[((size_t)at.i * g.H + at.h) * b.width + gb] = y;
+}
+
+template <class T, int DP>
+int go_mass(const CUtensorMap &km, const CUtensorMap &qm, const MassGeo &g, const PagesDev &p, const BatchDev &b,
+            const MassDev &a, const SplitDev &sp, cudaStream_t s)
+{
+    auto k = mass_tile_kernel<T, DP>;
+    const size_t smem = MassCfg<DP>::tiles + sizeof(MassShared);
+    OKV_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    k<<<sp.ctas, kMassThreads, smem, s>>>(km, qm, g, p, b, a, sp, p.head_b == 0);
+    note_launches(1);
+    OKV_CUDA_TRY(cudaGetLastError());
+    if (sp.ctas > 1) {
+        OKV_CUDA_TRY(launch_after(mass_join_kernel, sp.ctas - 1, 128, 0, s, g, p, b, a, sp));
+        note_launches(1);
+    }
+    return ORCHKV_OK;
+}
+
 }  // namespace
 
-bool page_map(CUtensorMap *m, const PagesDev &p, const char *base, int dtype)
+namespace {
+
+CUresult encode_map(CUtensorMap *m, int dtype, int rank, const char *base, const cuuint64_t *dims,
+                    const cuuint64_t *strides, const cuuint32_t *box)
 {
     typedef CUresult (*encode_t)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
@@ -475,18 +1001,34 @@ bool page_map(CUtensorMap *m, const PagesDev &p, const char *base, int dtype)
             f = nullptr;
         return (encode_t)f;
     }();
-    if (!encode) return false;
+    if (!encode) return CUDA_ERROR_NOT_SUPPORTED;
+    const cuuint32_t one[4] = {1, 1, 1, 1};
+    return encode(m, dtype == DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                  rank, (void *)base, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+}  // namespace
+
+bool page_map(CUtensorMap *m, const PagesDev &p, const char *base, int dtype)
+{
     // pages of one head: a head axis of one entry
     const bool by_head = p.head_b == 0;
     const cuuint64_t dims[4] = {p.D, p.bs.d, by_head ? 1 : p.H, p.n_pages};
     const cuuint64_t strides[3] = {(cuuint64_t)p.tok_b, (cuuint64_t)(by_head ? p.tok_b : p.head_b),
                                    (cuuint64_t)p.page_b};
     const cuuint32_t box[4] = {64, p.bs.d < 128 ? p.bs.d : 128, 1, 1};
-    const cuuint32_t one[4] = {1, 1, 1, 1};
-    return encode(m, dtype == DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                  4, (void *)base, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return encode_map(m, dtype, 4, base, dims, strides, box) == CUDA_SUCCESS;
+}
+
+bool rows_map(CUtensorMap *m, const RowsDev &q, uint32_t D, uint32_t Hq, uint32_t rows, uint32_t G,
+              uint32_t toks, int dtype)
+{
+    const cuuint64_t dims[3] = {D, Hq, rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)q.head_b, (cuuint64_t)q.row_b};
+    const cuuint32_t box[3] = {64, G, toks};
+    return encode_map(m, dtype, 3, q.p, dims, strides, box) == CUDA_SUCCESS;
 }
 
 // 16-bit pages whose tokens fill whole boxes; a scale that keeps the order of
@@ -495,6 +1037,34 @@ bool attend_tile_takes(const PagesDev &p, int dtype, float sl2)
 {
     return dtype != DTYPE_FP32 && pages_tile(p) && sl2 > 0.f && p.page_b >= 0 && p.head_b >= 0 && p.tok_b > 0 &&
            p.page_b < (1ll << 40) && p.head_b < (1ll << 40) && p.tok_b < (1ll << 40);
+}
+
+// Besides: whole blocks in a unit's 256 keys, a group of at most 128 heads,
+// row strides that a tensor map takes.
+bool mass_tile_takes(const PagesDev &p, int dtype, float sl2, const RowsDev &q, uint32_t G)
+{
+    return attend_tile_takes(p, dtype, sl2) && kMK % p.bs.d == 0 && G <= 128 && q.head_b > 0 && q.row_b > 0 &&
+           q.head_b < (1ll << 40) && q.row_b < (1ll << 40);
+}
+
+uint32_t mass_tile_ctas(unsigned long long units, unsigned long long rows)
+{
+    const unsigned long long tiles = units * ((rows + 63) / 64);
+    return (uint32_t)(tiles < 148 ? tiles : 148);
+}
+
+int launch_mass_tile(int dtype, const PagesDev &p, const BatchDev &b, const MassDev &a, const ClassDev &cl,
+                     const SplitDev &sp, cudaStream_t s)
+{
+    const MassGeo g = {a.G, p.H, a.window, cl.min_rows, 128 / a.G};
+    CUtensorMap km, qm;
+    if (!page_map(&km, p, p.k, dtype) || !rows_map(&qm, a.q, p.D, a.Hq, b.rows, a.G, g.toks, dtype))
+        return ORCHKV_ERR_CUDA;
+    if (dtype == DTYPE_BF16)
+        return p.D <= 64 ? go_mass<__nv_bfloat16, 64>(km, qm, g, p, b, a, sp, s)
+                         : go_mass<__nv_bfloat16, 128>(km, qm, g, p, b, a, sp, s);
+    return p.D <= 64 ? go_mass<__half, 64>(km, qm, g, p, b, a, sp, s)
+                     : go_mass<__half, 128>(km, qm, g, p, b, a, sp, s);
 }
 
 uint32_t attend_tile_ctas(unsigned long long units, unsigned long long keys)

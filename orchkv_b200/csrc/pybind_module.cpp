@@ -69,6 +69,16 @@ static orchkv_attend_args_t attend_of(const py::tuple &t)
     return a;
 }
 
+static orchkv_mass_args_t mass_of(const py::tuple &q, const py::tuple &t)
+{
+    orchkv_mass_args_t a = {};
+    a.q = rows_of(q);
+    a.n_q_heads = t[0].cast<uint32_t>();
+    a.scale = t[1].cast<float>();
+    a.window = t[2].cast<uint32_t>();
+    return a;
+}
+
 PYBIND11_MODULE(orchkv_core, m)
 {
     m.doc() = "OrchKvCache (B200): tiered KV-cache scheduling and migration on sm_100a";
@@ -532,20 +542,23 @@ PYBIND11_MODULE(orchkv_core, m)
           py::arg("pages"), py::arg("batch"), py::arg("q"), py::arg("out"), py::arg("lse_ptr"),
           py::arg("args"), py::arg("workspace_ptr"), py::arg("workspace_bytes"),
           py::arg("stream") = 0);
+    m.def("paged_block_mass_workspace",
+          [](const orchkv_pages_t &pg, const py::tuple &batch, const py::tuple &q, const py::tuple &x) {
+              const orchkv_batch_t b = batch_of(batch);
+              const orchkv_mass_args_t a = mass_of(q, x);
+              return orchkv_paged_block_mass_workspace(&pg, &b, &a);
+          },
+          py::arg("pages"), py::arg("batch"), py::arg("q"), py::arg("args"));
     m.def("paged_block_mass",
           [](const orchkv_pages_t &pg, const py::tuple &batch, const py::tuple &q, uintptr_t lse,
-             uintptr_t mass, const py::tuple &x, uintptr_t stream) {
+             uintptr_t mass, const py::tuple &x, uintptr_t ws, size_t bytes, uintptr_t stream) {
               const orchkv_batch_t b = batch_of(batch);
-              const orchkv_attend_args_t t = attend_of(x);
-              orchkv_mass_args_t a = {};
-              a.q = rows_of(q);
+              orchkv_mass_args_t a = mass_of(q, x);
               a.lse = P<const float>(lse);
               a.mass = P<float>(mass);
-              a.n_q_heads = t.n_q_heads;
-              a.scale = t.scale;
-              a.window = t.window;
-              return orchkv_paged_block_mass(&pg, &b, &a, P<void>(stream));
+              return orchkv_paged_block_mass(&pg, &b, &a, P<void>(ws), bytes, P<void>(stream));
           },
           py::arg("pages"), py::arg("batch"), py::arg("q"), py::arg("lse_ptr"),
-          py::arg("mass_ptr"), py::arg("args"), py::arg("stream") = 0);
+          py::arg("mass_ptr"), py::arg("args"), py::arg("workspace_ptr"), py::arg("workspace_bytes"),
+          py::arg("stream") = 0);
 }

@@ -342,5 +342,8 @@ class PagedKV:
                     or out.get_device() != self._dev):
                 raise ValueError(f"out must be fp32 {list(shape)}, contiguous, on the pages' device")
         args = (hq, self.head_dim ** -0.5 if scale is None else scale, window)
-        self._call(self._C.paged_block_mass, pg, batch, qa, lse.data_ptr(), out.data_ptr(), args)
+        need = self._C.paged_block_mass_workspace(pg, batch, qa, args)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        self._call(self._C.paged_block_mass, pg, batch, qa, lse.data_ptr(), out.data_ptr(), args,
+                   ws.data_ptr() if need else 0, need)
         return out

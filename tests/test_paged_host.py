@@ -37,7 +37,7 @@ def call(**kw):
         append=lambda: L.orchkv_paged_append(C.byref(pg), C.byref(b), C.byref(ap), None),
         attend=lambda: L.orchkv_paged_attend(C.byref(pg), C.byref(b), C.byref(at), v["ws"],
                                              max(0, need - v["short"]), None),
-        mass=lambda: L.orchkv_paged_block_mass(C.byref(pg), C.byref(b), C.byref(ms), None))
+        mass=lambda: L.orchkv_paged_block_mass(C.byref(pg), C.byref(b), C.byref(ms), v["ws"], 1 << 30, None))
 
 
 EVERY = ("append", "attend", "mass")
