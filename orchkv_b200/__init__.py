@@ -12,6 +12,8 @@ Callers of the reference's Python layer have B200 counterparts with the
 same interfaces: ``fast_manager.FastKVCacheManager``,
 ``kvcache_manager.KVCacheManager``, ``vllm_connector.OrchKvOffloadingConnector``
 and ``attention_hook.AttentionScoreCollector`` / ``AttentionHookManager``.
+``paged.PagedKV`` has the operators over a paged cache itself: appending
+rotated tokens, attending over the pages, and the blocks' attention mass.
 
 There is no CPU fallback: if the library has not been built, the first call
 into it (``lib()`` or ``core()``) raises.
@@ -40,24 +42,34 @@ def lib() -> C.CDLL:
     return _lib.load()
 
 
-_CORE = None
+_MODULES = {}
+
+
+def _extension(name: str, path: str):
+    """The in-tree extension module `name`, registered as a top-level module."""
+    if name not in _MODULES:
+        if not os.path.exists(path):
+            raise ImportError(f"{path} not built: run `python -m orchkv_b200.build`")
+        loader = importlib.machinery.ExtensionFileLoader(name, path)
+        spec = importlib.util.spec_from_file_location(name, path, loader=loader)
+        mod = importlib.util.module_from_spec(spec)
+        loader.exec_module(mod)
+        sys.modules[name] = mod
+        _MODULES[name] = mod
+    return _MODULES[name]
 
 
 def core():
     """Load the orchkv_core extension and register it as ``orchkv_core``."""
-    global _CORE
-    if _CORE is None:
-        from .build import core_module_path
-        path = core_module_path(_lib.LIB_DIR)
-        if not os.path.exists(path):
-            raise ImportError(f"{path} not built: run `python -m orchkv_b200.build`")
-        loader = importlib.machinery.ExtensionFileLoader("orchkv_core", path)
-        spec = importlib.util.spec_from_file_location("orchkv_core", path, loader=loader)
-        mod = importlib.util.module_from_spec(spec)
-        loader.exec_module(mod)
-        sys.modules["orchkv_core"] = mod
-        _CORE = mod
-    return _CORE
+    from .build import core_module_path
+    return _extension("orchkv_core", core_module_path(_lib.LIB_DIR))
+
+
+def torch_ops():
+    """Load the orchkv_torch extension (the paged operators on torch tensors)."""
+    import torch  # noqa: F401  (its libraries are loaded first)
+    from .build import torch_module_path
+    return _extension("orchkv_torch", torch_module_path(_lib.LIB_DIR))
 
 
 def make_config(gpu_pool_bytes, dram_pool_bytes, tokens_per_block=64, d_head=128, dtype=0,

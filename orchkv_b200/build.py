@@ -8,6 +8,8 @@ Outputs (in-tree, git-ignored, shipped with the working tree):
     orchkv_b200/liborchkv_b200.so               C ABI: orchkv_* and tm_*
     orchkv_b200/orchkv_core<ext-suffix>.so      pybind11 module (same names as
                                                 the reference binding)
+    orchkv_b200/orchkv_torch<ext-suffix>.so     the paged operators on torch
+                                                tensors (orchkv_b200/paged.py)
     orchkv_b200/_checked/...                    the same two, built with
                                                 -DOKV_CHECKED (--checked;
                                                 selected by ORCHKV_CHECKED=1)
@@ -46,6 +48,11 @@ CHECKED = os.path.join(PKG, "_checked")        # the checked build's library and
 def core_module_path(directory: str = PKG) -> str:
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
     return os.path.join(directory, "orchkv_core" + suffix)
+
+
+def torch_module_path(directory: str = PKG) -> str:
+    suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
+    return os.path.join(directory, "orchkv_torch" + suffix)
 
 
 def _headers():
@@ -108,6 +115,22 @@ def build(clean: bool = False, verbose: bool = False, checked: bool = False) -> 
               "-I" + py_inc, "-I" + pybind11.get_include(), "-I" + INCLUDE,
               "-I/usr/local/cuda/include", src, "-o", mod, "-L" + out_dir,
               "-l:liborchkv_b200.so", "-Wl,-rpath,$ORIGIN"])
+
+    # torch module of the paged operators, with the installed torch's headers
+    mod = torch_module_path(out_dir)
+    src = os.path.join(CSRC, "torch_ops.cpp")
+    if clean or _newer(mod, [src, lib] + hdrs):
+        import torch
+        from torch.utils.cpp_extension import include_paths
+        py_inc = sysconfig.get_paths()["include"]
+        tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
+        abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+        _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+              f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=orchkv_torch",
+              "-I" + INCLUDE] + [x for p in include_paths() for x in ("-isystem", p)] +
+             ["-isystem", py_inc, "-isystem", "/usr/local/cuda/include", src, "-o", mod,
+              "-L" + out_dir, "-l:liborchkv_b200.so", "-L" + tlib, "-lc10", "-lc10_cuda", "-ltorch_cpu",
+              "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
 
 
 def main(argv=None):

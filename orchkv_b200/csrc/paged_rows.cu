@@ -393,13 +393,13 @@ int attend_d(const PagesDev &p, const BatchDev &b, const AttendDev &a, const Cla
 {
     const Geo g = {kR, kKeys, a.G, p.H, a.window, cl.min_rows, cl.max_rows};
     auto k = attend_rows_kernel<T, DP>;
-    OKV_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)RowsCfg<DP>::smem));
+    static std::atomic<uint64_t> done;
+    OKV_CUDA_TRY(allow_smem(k, RowsCfg<DP>::smem, done));
     k<<<sp.ctas, kW * 32, RowsCfg<DP>::smem, s>>>(g, p, b, a, sp);
     note_launches(1);
     OKV_CUDA_TRY(cudaGetLastError());
     if (sp.ctas > 1) {
-        OKV_CUDA_TRY(launch_after(join_kernel<T, 128>, sp.ctas - 1, 128, 0, s, g, p, b, a, sp));
+        OKV_CUDA_TRY(launch_after(join_kernel<T, 128>, sp.ctas - 1, 128, 0, s, g, p, b, a, sp, 1u));
         note_launches(1);
     }
     return ORCHKV_OK;
@@ -422,7 +422,8 @@ int mass_d(const PagesDev &p, const BatchDev &b, const MassDev &a, const ClassDe
     if (grid > 0x7FFFFFFFull) return ORCHKV_ERR_INVALID;
     auto k = mass_rows_kernel<T, DP>;
     const size_t smem = (size_t)kW * kMassStages * 16 * DP * 2;
-    OKV_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static std::atomic<uint64_t> done;
+    OKV_CUDA_TRY(allow_smem(k, smem, done));
     k<<<(unsigned)grid, kW * 32, smem, s>>>(g, p, b, a, per_item, run, groups);
     note_launches(1);
     OKV_CUDA_TRY(cudaGetLastError());

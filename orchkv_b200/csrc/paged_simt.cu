@@ -292,7 +292,7 @@ int attend(const PagesDev &p, const BatchDev &b, const AttendDev &a, const Class
     note_launches(1);
     OKV_CUDA_TRY(cudaGetLastError());
     if (sp.ctas > 1) {
-        OKV_CUDA_TRY(launch_after(join_kernel<T, 128>, sp.ctas - 1, 128, 0, s, g, p, b, a, sp));
+        OKV_CUDA_TRY(launch_after(join_kernel<T, 128>, sp.ctas - 1, 128, 0, s, g, p, b, a, sp, 1u));
         note_launches(1);
     }
     return ORCHKV_OK;

@@ -13,11 +13,21 @@
 // the same result for the same lengths every time.
 #pragma once
 
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace okv {
 
 typedef unsigned long long ull;
+
+// 64-bit quotient; the values of small calls fit 32 bits, where a division
+// takes a fraction of the time.
+__device__ __forceinline__ ull quot(ull x, ull y)
+{
+    if (((x | y) >> 32) == 0) return (uint32_t)x / (uint32_t)y;
+    return x / y;
+}
 
 struct Geo {                     // what the division depends on besides the lengths
     uint32_t R, KT, G, H, window;
@@ -75,11 +85,13 @@ __device__ __forceinline__ Pos inside(const Geo &g, const SeqDev &s, uint32_t i,
     const ull U = weight_before(base, slope, RT);
     Pos p;
     p.i = i;
-    p.h = (uint32_t)(x / U);
+    p.h = (uint32_t)quot(x, U);
     const ull y = x - (ull)p.h * U;
     ull rt;
-    if (slope == 0) {
-        rt = y / base;
+    if (RT == 1) {
+        rt = 0;
+    } else if (slope == 0) {
+        rt = quot(y, base);
     } else {
         const double bb = (double)base - 0.5 * (double)slope;
         rt = (ull)((sqrt(bb * bb + 2.0 * (double)slope * (double)y) - bb) / (double)slope);
@@ -91,7 +103,7 @@ __device__ __forceinline__ Pos inside(const Geo &g, const SeqDev &s, uint32_t i,
     uint32_t first, nt;
     key_tiles(g, s, p.rt, &first, &nt);
     const ull z = y - weight_before(base, slope, rt), w = base + slope * rt;
-    p.t = (uint32_t)(z * nt / w);
+    p.t = (uint32_t)quot(z * nt, w);
     return p;
 }
 
@@ -143,6 +155,32 @@ template <int NT, class Weight, class Where>
 __device__ void find_share(const BatchDev &b, uint32_t bs, uint32_t c, uint32_t C, SplitShared *sh, Pos *from,
                            Pos *to, ull *W, Weight weight, Where where)
 {
+    if (b.n <= 32) {
+        // every warp for itself, a lane a sequence: no barriers
+        const uint32_t lane = threadIdx.x & 31;
+        const ull w = lane < b.n ? weight(lane) : 0;
+        ull inc = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const ull u = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+            if (lane >= o) inc += u;
+        }
+        const ull total = __shfl_sync(0xFFFFFFFFu, inc, 31);
+        *W = total;
+        if (total == 0) return;
+        const ull share = quot(total + C - 1, C);
+        Pos *out[2] = {from, to};
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const ull x = min((c + k) * share, total);
+            const uint32_t in = __ballot_sync(0xFFFFFFFFu, x >= inc - w && x < inc);
+            const uint32_t i = in ? __ffs(in) - 1 : 0;
+            const ull off = x - __shfl_sync(0xFFFFFFFFu, inc - w, i);
+            if (k == 1 && threadIdx.x == 0) sh->off[1] = off;
+            *out[k] = in ? where(load_seq(b, bs, i), i, off) : Pos{b.n, 0, 0, 0};
+        }
+        return;
+    }
     ull sum = 0, one = 0;
     for (uint32_t i = threadIdx.x; i < b.n; i += NT) {
         one = weight(i);
@@ -153,7 +191,7 @@ __device__ void find_share(const BatchDev &b, uint32_t bs, uint32_t c, uint32_t 
     *W = total;
     if (total == 0) return;
     // shares of ceil(total / C): the last ones may be empty
-    const ull share = (total + C - 1) / C;
+    const ull share = quot(total + C - 1, C);
     const ull x[2] = {min(c * share, total), min((c + 1) * share, total)};
     if (threadIdx.x == 0) sh->seq[0] = sh->seq[1] = b.n;
     __syncthreads();
@@ -233,76 +271,124 @@ __device__ __forceinline__ float *slot_of(float *ws, uint32_t slot, uint32_t R, 
 }
 __host__ __device__ inline size_t slot_floats(uint32_t R, uint32_t D) { return (size_t)R * (D + 2); }
 
+// The slots of the pieces of the unit that boundary c (at position `at`, offset
+// `off` of its sequence) is the first to cut, in key order: slot 2(c-1)+1 for
+// the unit's start, held by CTA c - 1, then 2c, 2(c+1), ...; ~0 for an empty
+// piece.  A thread takes a boundary.  Returns their number (at most kMaxPieces).
+constexpr uint32_t kMaxPieces = 600;
+template <int NT, class Where>
+__device__ uint32_t find_pieces(const BatchDev &b, uint32_t c, uint32_t C, const Pos &at, ull off, ull share,
+                                ull seqW, uint32_t nt, uint32_t *slots, Where where)
+{
+    constexpr uint32_t kOut = 0xFFFFFFFFu;
+    __shared__ uint32_t t_s[NT + 1];
+    __shared__ uint32_t n_s;
+    if (threadIdx.x == 0) {
+        t_s[0] = at.t;
+        slots[0] = 2 * (c - 1) + 1;
+    }
+    uint32_t n = 1;
+    for (uint32_t k0 = 0;; k0 += NT) {
+        const uint32_t cc = c + k0 + threadIdx.x;          // a piece: boundaries cc and cc + 1
+        const ull x = off + (ull)(k0 + threadIdx.x + 1) * share;
+        uint32_t t = kOut;
+        if (cc + 1 < C && x < seqW) {
+            const Pos nx = where(x);
+            if (same_unit(nx, at)) t = nx.t;
+        }
+        t_s[threadIdx.x + 1] = t;
+        __syncthreads();
+        const uint32_t from = t_s[threadIdx.x], to = t == kOut ? nt : t;
+        if (from != kOut && cc < C && 1 + k0 + threadIdx.x < kMaxPieces) {
+            slots[1 + k0 + threadIdx.x] = to > from ? 2 * cc : kOut;
+            if (t == kOut) n_s = 2 + k0 + threadIdx.x;     // the last one
+        }
+        const bool more = t_s[NT] != kOut;
+        __syncthreads();
+        if (!more) break;
+        if (threadIdx.x == 0) t_s[0] = t_s[NT];
+        __syncthreads();
+        n += NT;
+    }
+    __syncthreads();
+    return min(n_s, kMaxPieces);
+}
+
 // The pieces of every cut unit into its rows.  Block c looks at boundary c: it
-// works if that is the first boundary inside a unit.  Pieces lie in slot
-// 2c'+1 (the unit's start, held by CTA c' = c - 1) and in slots 2c, 2c+2, ...
+// works if that is the first boundary inside a unit (`parts` blocks share the
+// unit's rows).  All but the partials is known beforehand and found out while
+// the kernel in front still runs.
 template <class T, int NT>
 __global__ void __launch_bounds__(NT)
-join_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp)
+join_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint32_t parts)
 {
-    cudaGridDependencySynchronize();
     __shared__ SplitShared sh;
-    const uint32_t c = blockIdx.x + 1;
+    __shared__ uint32_t slots[kMaxPieces];
+    const uint32_t c = blockIdx.x / parts + 1, part = blockIdx.x % parts;
     Pos prev, at;
     ull W;
     find_share<NT>(g, b, p.bs.d, c - 1, sp.ctas, &sh, &prev, &at, &W);
-    if (W == 0 || at.i >= b.n || at.t == 0) return;
-    if (same_unit(prev, at) && prev.t > 0) return;
+    // (no block ends before the kernel in front: the next launch counts on that)
+    if (W == 0 || at.i >= b.n || at.t == 0 || (same_unit(prev, at) && prev.t > 0)) {
+        cudaGridDependencySynchronize();
+        return;
+    }
+    __syncthreads();
     const SeqDev s = load_seq(b, p.bs.d, at.i);
     uint32_t first, nt;
     key_tiles(g, s, at.rt, &first, &nt);
-    // the boundaries after c that fall into the unit, as offsets of the sequence
-    const ull share = (W + sp.ctas - 1) / sp.ctas;
-    __shared__ uint32_t slots[1024];
-    __shared__ uint32_t n_slots;
-    if (threadIdx.x == 0) {
-        uint32_t k = 0;
-        slots[k++] = 2 * (c - 1) + 1;
-        ull off = sh.off[1];
-        Pos cur = at;
-        ull base, slope;
-        weights(g, s, &base, &slope);
-        const ull seqW = g.H * weight_before(base, slope, row_tiles(g, s));
-        for (uint32_t cc = c; cc < sp.ctas; cc++) {
-            off += share;
-            Pos nx = off < seqW && cc + 1 < sp.ctas ? inside(g, s, at.i, off) : Pos{b.n, 0, 0, 0};
-            const bool in = same_unit(nx, at);
-            if ((in ? nx.t : nt) > cur.t && k < 1024) slots[k++] = 2 * cc;
-            if (!in) break;
-            cur = nx;
-        }
-        n_slots = k;
-    }
-    __syncthreads();
-    const uint32_t K = n_slots, D = p.D, R = g.R;
-    const uint32_t d4 = D / 4;
-    for (uint32_t e = threadIdx.x; e < R * d4; e += NT) {
+    ull base, slope;
+    weights(g, s, &base, &slope);
+    const ull seqW = g.H * weight_before(base, slope, row_tiles(g, s));
+    const uint32_t K = find_pieces<NT>(b, c, sp.ctas, at, sh.off[1], quot(W + sp.ctas - 1, sp.ctas), seqW, nt,
+                                       slots, [&](ull x) { return inside(g, s, at.i, x); });
+    const uint32_t D = p.D, R = g.R, d4 = D / 4;
+    const uint32_t live = min(R, (uint32_t)s.m * g.G - at.rt * R);
+    const uint32_t each = (live + parts - 1) / parts, r_end = min(live, (part + 1) * each);
+    cudaGridDependencySynchronize();
+    for (uint32_t e = part * each * d4 + threadIdx.x; e < r_end * d4; e += NT) {
         const uint32_t rr = e / d4, d = (e - rr * d4) * 4;
-        const RowInfo ri = row_info(g, s, at.h, at.rt * R + rr);
-        if (ri.row < 0) continue;
-        float M = -INFINITY;
-        for (uint32_t k = 0; k < K; k++) M = fmaxf(M, slot_of(sp.ws, slots[k], R, D)[rr]);
-        const float Ms = M == -INFINITY ? 0.f : M;
-        float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+        float M = -INFINITY, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
         for (uint32_t k = 0; k < K; k++) {
+            if (slots[k] == 0xFFFFFFFFu) continue;
             const float *sl = slot_of(sp.ws, slots[k], R, D);
-            const float w = exp2f(sl[rr] - Ms);
-            L += w * sl[R + rr];
+            const float m = sl[rr], l = sl[R + rr];
             const float4 v = *(const float4 *)(sl + 2 * R + (size_t)rr * D + d);
+            const float nm = fmaxf(M, m), ms = nm == -INFINITY ? 0.f : nm;
+            const float f = exp2f(M - ms), w = exp2f(m - ms);
+            M = nm;
+            L = L * f + w * l;
             // a piece without an attended token holds zeros
-            o[0] += w * v.x;
-            o[1] += w * v.y;
-            o[2] += w * v.z;
-            o[3] += w * v.w;
+            o[0] = o[0] * f + w * v.x;
+            o[1] = o[1] * f + w * v.y;
+            o[2] = o[2] * f + w * v.z;
+            o[3] = o[3] * f + w * v.w;
         }
+        const float Ms = M == -INFINITY ? 0.f : M;
         const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
-        T *dst = (T *)(a.out.p + (long long)ri.row * a.out.row_b + (long long)ri.head * a.out.head_b) + d;
+        const RowInfo ri = row_info(g, s, at.h, at.rt * R + rr);
+        T y[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) dst[j] = from_f<T>(o[j] * inv);
+        for (int j = 0; j < 4; j++) y[j] = from_f<T>(o[j] * inv);
+        char *dst = a.out.p + (long long)ri.row * a.out.row_b + (long long)ri.head * a.out.head_b + d * sizeof(T);
+        if (sizeof(T) == 4) *(uint4 *)dst = *(const uint4 *)y;
+        else *(uint2 *)dst = *(const uint2 *)y;
         if (a.lse && d == 0)
             a.lse[(size_t)ri.row * a.Hq + ri.head] =
                 L > 0.f ? (Ms + log2f(L)) * 0.69314718055994531f : L == 0.f ? -INFINITY : L;
     }
+}
+
+// Dynamic shared memory over 48 KB, once a kernel and device.
+template <class K> cudaError_t allow_smem(K k, size_t bytes, std::atomic<uint64_t> &done)
+{
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && done.load() >> dev & 1)) return e;
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && dev < 64) done |= 1ull << dev;
+    return e;
 }
 
 // A launch that may begin before the one in front of it in the stream has

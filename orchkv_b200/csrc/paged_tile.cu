@@ -448,12 +448,13 @@ int go(const CUtensorMap &km, const CUtensorMap &vm, const PagesDev &p, const Ba
 {
     const Geo g = {kR, kK, a.G, p.H, a.window, cl.min_rows, cl.max_rows};
     auto k = attend_tile_kernel<T, DP>;
-    OKV_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TileCfg<DP>::smem));
+    static std::atomic<uint64_t> done;
+    OKV_CUDA_TRY(allow_smem(k, TileCfg<DP>::smem, done));
     k<<<sp.ctas, kThreads, TileCfg<DP>::smem, s>>>(km, vm, g, p, b, a, sp, p.head_b == 0);
     note_launches(1);
     OKV_CUDA_TRY(cudaGetLastError());
     if (sp.ctas > 1) {
-        OKV_CUDA_TRY(launch_after(join_kernel<T, 512>, sp.ctas - 1, 512, 0, s, g, p, b, a, sp));
+        OKV_CUDA_TRY(launch_after(join_kernel<T, 256>, (sp.ctas - 1) * 8, 256, 0, s, g, p, b, a, sp, 8u));
         note_launches(1);
     }
     return ORCHKV_OK;
@@ -545,7 +546,7 @@ __device__ __forceinline__ Pos mass_inside(const MassGeo &g, const SeqDev &s, ui
     const ull U = mass_before(g, s, q, q.kn);
     Pos p;
     p.i = i;
-    p.h = (uint32_t)(x / U);
+    p.h = (uint32_t)quot(x, U);
     const ull y = x - (ull)p.h * U;
     uint32_t lo = 0, hi = q.kn;                        // the last k with before(k) <= y
     while (hi - lo > 1) {
@@ -555,7 +556,7 @@ __device__ __forceinline__ Pos mass_inside(const MassGeo &g, const SeqDev &s, ui
     }
     p.rt = lo;
     const ull z = y - mass_before(g, s, q, lo), w = mass_before(g, s, q, lo + 1) - mass_before(g, s, q, lo);
-    p.t = (uint32_t)(z * mass_tiles(g, s, q, lo) / w);
+    p.t = (uint32_t)quot(z * mass_tiles(g, s, q, lo), w);
     return p;
 }
 
@@ -935,34 +936,33 @@ mass_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 __global__ void __launch_bounds__(128)
 mass_join_kernel(MassGeo g, PagesDev p, BatchDev b, MassDev a, SplitDev sp)
 {
-    cudaGridDependencySynchronize();
     __shared__ SplitShared sh;
+    __shared__ uint32_t slots[kMaxPieces];
     const uint32_t c = blockIdx.x + 1;
     Pos prev, at;
     ull W;
     find_share<128>(b, p.bs.d, c - 1, sp.ctas, &sh, &prev, &at, &W,
                     [&](uint32_t i) { return mass_weight(g, b, p.bs.d, i); },
                     [&](const SeqDev &s, uint32_t i, ull x) { return mass_inside(g, s, i, x); });
-    if (W == 0 || at.i >= b.n || at.t == 0) return;
-    if (same_unit(prev, at) && prev.t > 0) return;
+    // (no block ends before the kernel in front: the next launch counts on that)
+    if (W == 0 || at.i >= b.n || at.t == 0 || (same_unit(prev, at) && prev.t > 0)) {
+        cudaGridDependencySynchronize();
+        return;
+    }
+    __syncthreads();
     const SeqDev s = load_seq(b, p.bs.d, at.i);
     const MassSeq q = mass_seq(g, s);
-    const ull share = (W + sp.ctas - 1) / sp.ctas, seqW = g.H * mass_before(g, s, q, q.kn);
-    const uint32_t nb = kMK / p.bs.d, lb = threadIdx.x;
-    const uint32_t gb = (q.kf + at.rt) * nb + lb, nt = mass_tiles(g, s, q, at.rt);
+    const uint32_t K = find_pieces<128>(b, c, sp.ctas, at, sh.off[1], quot(W + sp.ctas - 1, sp.ctas),
+                                        g.H * mass_before(g, s, q, q.kn), mass_tiles(g, s, q, at.rt), slots,
+                                        [&](ull x) { return mass_inside(g, s, at.i, x); });
+    const uint32_t nb = kMK / p.bs.d, lb = threadIdx.x, gb = (q.kf + at.rt) * nb + lb;
+    cudaGridDependencySynchronize();
+    if (lb >= nb || gb >= b.width) return;
     float y = 0.f;
-    if (lb < nb) y = sp.ws[(size_t)(2 * (c - 1) + 1) * kMassSlot + lb];
-    ull off = sh.off[1];
-    Pos cur = at;
-    for (uint32_t cc = c; cc < sp.ctas; cc++) {
-        off += share;
-        const Pos nx = off < seqW && cc + 1 < sp.ctas ? mass_inside(g, s, at.i, off) : Pos{b.n, 0, 0, 0};
-        const bool in = same_unit(nx, at);
-        if ((in ? nx.t : nt) > cur.t && lb < nb) y += sp.ws[(size_t)2 * cc * kMassSlot + lb];
-        if (!in) break;
-        cur = nx;
-    }
-    if (lb < nb && gb < b.width) a.mass[((size_t)at.i * g.H + at.h) * b.width + gb] = y;
+#pragma unroll 4
+    for (uint32_t k = 0; k < K; k++)
+        if (slots[k] != 0xFFFFFFFFu) y += sp.ws[(size_t)slots[k] * kMassSlot + lb];
+    a.mass[((size_t)at.i * g.H + at.h) * b.width + gb] = y;
 }
 
 template <class T, int DP>
@@ -971,7 +971,8 @@ int go_mass(const CUtensorMap &km, const CUtensorMap &qm, const MassGeo &g, cons
 {
     auto k = mass_tile_kernel<T, DP>;
     const size_t smem = MassCfg<DP>::tiles + sizeof(MassShared);
-    OKV_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static std::atomic<uint64_t> done;
+    OKV_CUDA_TRY(allow_smem(k, smem, done));
     k<<<sp.ctas, kMassThreads, smem, s>>>(km, qm, g, p, b, a, sp, p.head_b == 0);
     note_launches(1);
     OKV_CUDA_TRY(cudaGetLastError());

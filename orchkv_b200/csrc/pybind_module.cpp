@@ -19,7 +19,6 @@
 #include <vector>
 
 #include "orchkv/orchkv_api.h"
-#include "orchkv/paged_ops.h"
 #include "orchkv/tiered_manager.h"
 
 namespace py = pybind11;
@@ -34,49 +33,6 @@ static std::vector<kv_request_ctx_t *> ctx_list(const std::vector<uintptr_t> &v)
     std::vector<kv_request_ctx_t *> out(v.size());
     for (size_t i = 0; i < v.size(); i++) out[i] = P<kv_request_ctx_t>(v[i]);
     return out;
-}
-
-// Arguments of the paged operators arrive as tuples of ints (pointers and
-// element strides), one a group, unpacked here.
-static uintptr_t word(const py::tuple &t, size_t i) { return t[i].cast<uintptr_t>(); }
-
-static orchkv_batch_t batch_of(const py::tuple &t)
-{
-    orchkv_batch_t b;
-    b.table = P<const int32_t>(word(t, 0));
-    b.table_seq_stride = t[1].cast<int64_t>();
-    b.table_head_stride = t[2].cast<int64_t>();
-    b.table_width = t[3].cast<uint32_t>();
-    b.n_seqs = t[4].cast<uint32_t>();
-    b.lens = P<const int32_t>(word(t, 5));
-    b.starts = P<const int32_t>(word(t, 6));
-    b.n_rows = t[7].cast<uint32_t>();
-    b.max_new = t[8].cast<uint32_t>();
-    return b;
-}
-
-static orchkv_rows_t rows_of(const py::tuple &t)
-{
-    return orchkv_rows_t{P<void>(word(t, 0)), t[1].cast<int64_t>(), t[2].cast<int64_t>()};
-}
-
-static orchkv_attend_args_t attend_of(const py::tuple &t)
-{
-    orchkv_attend_args_t a = {};
-    a.n_q_heads = t[0].cast<uint32_t>();
-    a.scale = t[1].cast<float>();
-    a.window = t[2].cast<uint32_t>();
-    return a;
-}
-
-static orchkv_mass_args_t mass_of(const py::tuple &q, const py::tuple &t)
-{
-    orchkv_mass_args_t a = {};
-    a.q = rows_of(q);
-    a.n_q_heads = t[0].cast<uint32_t>();
-    a.scale = t[1].cast<float>();
-    a.window = t[2].cast<uint32_t>();
-    return a;
 }
 
 PYBIND11_MODULE(orchkv_core, m)
@@ -485,80 +441,4 @@ PYBIND11_MODULE(orchkv_core, m)
           },
           py::arg("tm"), py::arg("k"), py::arg("threshold_to_gpu"), py::arg("threshold_to_dram"),
           py::arg("out_ptr"), py::arg("count_ptr"));
-
-    // ---- operators over paged caches (orchkv_b200/paged.py) ------------------
-    py::class_<orchkv_pages_t>(m, "Pages")
-        .def(py::init([](uintptr_t k, uintptr_t v, int64_t page, int64_t head, int64_t token,
-                         uint32_t n_pages, uint32_t page_tokens, uint32_t n_kv_heads, uint32_t d_head,
-                         int dtype) {
-                 return orchkv_pages_t{P<void>(k), P<void>(v), page, head, token, n_pages, page_tokens,
-                                       n_kv_heads, d_head, dtype};
-             }),
-             py::arg("k_ptr"), py::arg("v_ptr"), py::arg("page_stride"), py::arg("head_stride"),
-             py::arg("token_stride"), py::arg("n_pages"), py::arg("page_tokens"),
-             py::arg("n_kv_heads"), py::arg("d_head"), py::arg("dtype"));
-    m.def("paged_append",
-          [](const orchkv_pages_t &pg, const py::tuple &batch, const py::tuple &q,
-             const py::tuple &q_out, const py::tuple &k, const py::tuple &v, const py::tuple &x,
-             uintptr_t stream) {
-              const orchkv_batch_t b = batch_of(batch);
-              orchkv_append_args_t a = {};
-              a.q = rows_of(q);
-              a.q_out = rows_of(q_out);
-              a.k = rows_of(k);
-              a.v = rows_of(v);
-              a.n_q_heads = x[0].cast<uint32_t>();
-              a.rot_dim = x[1].cast<uint32_t>();
-              a.interleaved = x[2].cast<int>();
-              a.scale = x[3].cast<float>();
-              a.turns = P<const double>(word(x, 4));
-              a.positions = P<const void>(word(x, 5));
-              a.positions_64 = x[6].cast<int>();
-              a.q_norm = P<const void>(word(x, 7));
-              a.k_norm = P<const void>(word(x, 8));
-              a.eps = x[9].cast<float>();
-              return orchkv_paged_append(&pg, &b, &a, P<void>(stream));
-          },
-          py::arg("pages"), py::arg("batch"), py::arg("q"), py::arg("q_out"), py::arg("k"),
-          py::arg("v"), py::arg("args"), py::arg("stream") = 0);
-    m.def("paged_attend_workspace",
-          [](const orchkv_pages_t &pg, const py::tuple &batch, const py::tuple &x) {
-              const orchkv_batch_t b = batch_of(batch);
-              const orchkv_attend_args_t a = attend_of(x);
-              return orchkv_paged_attend_workspace(&pg, &b, &a);
-          },
-          py::arg("pages"), py::arg("batch"), py::arg("args"));
-    m.def("paged_attend",
-          [](const orchkv_pages_t &pg, const py::tuple &batch, const py::tuple &q,
-             const py::tuple &out, uintptr_t lse, const py::tuple &x, uintptr_t ws, size_t bytes,
-             uintptr_t stream) {
-              const orchkv_batch_t b = batch_of(batch);
-              orchkv_attend_args_t a = attend_of(x);
-              a.q = rows_of(q);
-              a.out = rows_of(out);
-              a.lse = P<float>(lse);
-              return orchkv_paged_attend(&pg, &b, &a, P<void>(ws), bytes, P<void>(stream));
-          },
-          py::arg("pages"), py::arg("batch"), py::arg("q"), py::arg("out"), py::arg("lse_ptr"),
-          py::arg("args"), py::arg("workspace_ptr"), py::arg("workspace_bytes"),
-          py::arg("stream") = 0);
-    m.def("paged_block_mass_workspace",
-          [](const orchkv_pages_t &pg, const py::tuple &batch, const py::tuple &q, const py::tuple &x) {
-              const orchkv_batch_t b = batch_of(batch);
-              const orchkv_mass_args_t a = mass_of(q, x);
-              return orchkv_paged_block_mass_workspace(&pg, &b, &a);
-          },
-          py::arg("pages"), py::arg("batch"), py::arg("q"), py::arg("args"));
-    m.def("paged_block_mass",
-          [](const orchkv_pages_t &pg, const py::tuple &batch, const py::tuple &q, uintptr_t lse,
-             uintptr_t mass, const py::tuple &x, uintptr_t ws, size_t bytes, uintptr_t stream) {
-              const orchkv_batch_t b = batch_of(batch);
-              orchkv_mass_args_t a = mass_of(q, x);
-              a.lse = P<const float>(lse);
-              a.mass = P<float>(mass);
-              return orchkv_paged_block_mass(&pg, &b, &a, P<void>(ws), bytes, P<void>(stream));
-          },
-          py::arg("pages"), py::arg("batch"), py::arg("q"), py::arg("lse_ptr"),
-          py::arg("mass_ptr"), py::arg("args"), py::arg("workspace_ptr"), py::arg("workspace_bytes"),
-          py::arg("stream") = 0);
 }

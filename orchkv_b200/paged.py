@@ -30,7 +30,7 @@ import math
 
 import torch
 
-from . import core
+from . import torch_ops
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
@@ -168,87 +168,10 @@ class PagedKV:
                   heads, sh[-1], k.dtype)
 
     def _set(self, device, k_ptr, v_ptr, strides, n_pages, tokens, heads, head_dim, dtype):
-        self._C = core()
-        self._dev = device
         self.n_pages, self.page_tokens, self.head_dim, self.dtype = n_pages, tokens, head_dim, dtype
         self.n_kv_heads = heads                   # None: as many as the call's tables have
-        self._args = (k_ptr, v_ptr) + strides + (n_pages, tokens)
-        self._align = 16 // dtype.itemsize
-        self._by_heads = {}
-
-    def _pages(self, heads: int):
-        _need(heads > 0, "a table of no heads")
-        pg = self._by_heads[heads] = self._C.Pages(*self._args, heads, self.head_dim,
-                                                   _DTYPES[self.dtype])
-        return pg
-
-    # -- argument checks -----------------------------------------------------
-
-    def _batch(self, table, lens, starts, rows, max_new):
-        """(pages handle, KV heads, the batch's arguments)."""
-        i32, dev, slab = torch.int32, self._dev, self.n_kv_heads is None
-        shape = table.shape
-        if table.dtype != i32 or lens.dtype != i32 or starts.dtype != i32:
-            raise ValueError("table, lens and starts must be int32")
-        if len(shape) != (3 if slab else 2):
-            raise ValueError("table must be [sequences, KV heads, width]" if slab
-                             else "table must be [sequences, width]")
-        n, width = shape[0], shape[-1]
-        if lens.shape != (n,) or starts.shape != (n + 1,):
-            raise ValueError("table, lens and starts must have n, n and n + 1 entries")
-        st = table.stride()
-        if st[-1] != 1 or not lens.is_contiguous() or not starts.is_contiguous():
-            raise ValueError("table rows, lens and starts must be contiguous")
-        if width == 0:
-            raise ValueError("a table of no blocks")
-        if table.get_device() != dev or lens.get_device() != dev or starts.get_device() != dev:
-            raise ValueError("every tensor must be on the pages' device")
-        if max_new is None:
-            max_new = rows
-        elif max_new < 0:
-            raise ValueError("max_new must not be negative")
-        heads = shape[1] if slab else self.n_kv_heads
-        pg = self._by_heads.get(heads) or self._pages(heads)
-        return pg, heads, (table.data_ptr(), st[0], st[1] if slab else 0, width, n, lens.data_ptr(),
-                           starts.data_ptr(), rows, max_new)
-
-    def _rows(self, x, name, heads=None, rows=None):
-        """Checks a row tensor; its (pointer, row stride, head stride)."""
-        shape = x.shape
-        if (len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads)
-                or (rows is not None and shape[0] != rows)):
-            raise ValueError(f"{name} must be [rows, heads, {self.head_dim}]"
-                             + ("" if heads is None else f" with {heads} heads")
-                             + ("" if rows is None else f" and {rows} rows"))
-        if x.dtype != self.dtype:
-            raise ValueError(f"{name} must be {self.dtype} as the pages are")
-        p, s, align = x.data_ptr(), x.stride(), self._align
-        if (s[2] != 1 or s[0] % align or s[1] % align or p % 16) and x.numel():
-            raise ValueError(f"{name}: heads must be contiguous, pointer and strides multiples of "
-                             "16 bytes")
-        if x.get_device() != self._dev:
-            raise ValueError(f"{name} must be on the pages' device")
-        if x.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{name} requires a gradient, which these operators do not have")
-        return p, s[0], s[1]
-
-    def _heads(self, hq, heads, window):
-        if hq == 0 or hq % heads:
-            raise ValueError(f"{hq} query heads do not share {heads} KV heads")
-        if window < 0:
-            raise ValueError("window must not be negative")
-
-    def _call(self, fn, *args):
-        dev = self._dev
-        if torch.cuda.current_device() == dev:
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
-        else:
-            with torch.cuda.device(dev):
-                rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
-        if rc != 0:
-            raise RuntimeError(f"orchkv_{fn.__name__} failed: {rc}")
-
-    # -- the operators -------------------------------------------------------
+        self._ops = torch_ops().Pages(device, k_ptr, v_ptr, *strides, n_pages, tokens, heads or 0,
+                                      head_dim, _DTYPES[dtype])
 
     def append(self, k, v, table, lens, starts, *, q=None, rotary: Rotary | None = None,
                positions=None, q_norm=None, k_norm=None, eps: float = 1e-6, q_out=None):
@@ -258,42 +181,10 @@ class PagedKV:
         [head_dim]: RMS norm of each head first.  positions [rows] (int32 or
         int64): where the rotation takes a token to be, by default its place
         in its sequence.  Rows behind the last sequence are left alone."""
-        rows = k.shape[0]
-        pg, heads, batch = self._batch(table, lens, starts, rows, None)
-        ka, va = self._rows(k, "k", heads), self._rows(v, "v", heads, rows)
-        qa = oa = (0, 0, 0)
-        hq = 0
-        if q is not None:
-            qa = self._rows(q, "q", None, rows)
-            hq = q.shape[1]
-            if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            oa = self._rows(q_out, "q_out", hq, rows)
-        else:
-            _need(q_out is None and q_norm is None, "q_out and q_norm go with q")
-        pos, pos64 = 0, 0
-        if positions is not None:
-            _need(positions.dtype in (torch.int32, torch.int64) and positions.shape == (rows,)
-                  and positions.is_contiguous() and positions.get_device() == self._dev,
-                  "positions must be int32 or int64 [rows], contiguous, on the pages' device")
-            pos, pos64 = positions.data_ptr(), int(positions.dtype == torch.int64)
-        norms = []
-        for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-            if w is not None:
-                if (w.shape != (self.head_dim,) or w.dtype != self.dtype or not w.is_contiguous()
-                        or w.get_device() != self._dev):
-                    raise ValueError(f"{name} must be [{self.head_dim}] {self.dtype}, contiguous, on "
-                                     "the pages' device")
-            norms.append(0 if w is None else w.data_ptr())
-        rot, inter, scale, turns = 0, 0, 1.0, 0
-        if rotary is not None:
-            rot, inter, scale = rotary.rotary_dim, int(rotary.interleaved), rotary.scale
-            _need(rot <= self.head_dim and rotary.turns.get_device() == self._dev,
-                  "rotary wider than a head, or on another device")
-            turns = rotary.turns.data_ptr()
-        self._call(self._C.paged_append, pg, batch, qa, oa, ka, va,
-                   (hq, rot, inter, scale, turns, pos, pos64, norms[0], norms[1], eps))
-        return q_out
+        turns, inter, scale = (None, False, 1.0) if rotary is None else (
+            rotary.turns, rotary.interleaved, rotary.scale)
+        return self._ops.append(k, v, table, lens, starts, q, turns, inter, scale, positions, q_norm,
+                                k_norm, eps, q_out)
 
     def attend(self, q, table, lens, starts, *, scale: float | None = None, window: int = 0,
                max_new: int | None = None, return_lse: bool = False, out=None):
@@ -304,21 +195,7 @@ class PagedKV:
         with nothing to attend to gets 0 and -inf.  max_new: the most new
         tokens of one sequence, if the caller knows it (decode: 1), lets the
         call leave out what only longer ones need."""
-        rows = q.shape[0]
-        qa = self._rows(q, "q")
-        hq = q.shape[1]
-        pg, heads, batch = self._batch(table, lens, starts, rows, max_new)
-        self._heads(hq, heads, window)
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        oa = self._rows(out, "out", hq, rows)
-        lse = torch.empty(rows, hq, dtype=torch.float32, device=q.device) if return_lse else None
-        args = (hq, self.head_dim ** -0.5 if scale is None else scale, window)
-        need = self._C.paged_attend_workspace(pg, batch, args)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        self._call(self._C.paged_attend, pg, batch, qa, oa, lse.data_ptr() if return_lse else 0, args,
-                   ws.data_ptr(), need)
-        return (out, lse) if return_lse else out
+        return self._ops.attend(q, table, lens, starts, scale, window, max_new, return_lse, out)
 
     def block_mass(self, q, lse, table, lens, starts, *, scale: float | None = None, window: int = 0,
                    max_new: int | None = None, out=None):
@@ -326,24 +203,4 @@ class PagedKV:
         width] fp32, the sum over the sequence's rows, the KV head's query
         heads and the block's tokens of exp(scale * q k - lse), with the lse
         that attend returned for the same arguments."""
-        rows = q.shape[0]
-        qa = self._rows(q, "q")
-        hq = q.shape[1]
-        pg, heads, batch = self._batch(table, lens, starts, rows, max_new)
-        self._heads(hq, heads, window)
-        if (lse.dtype != torch.float32 or lse.shape != (rows, hq) or not lse.is_contiguous()
-                or lse.get_device() != self._dev):
-            raise ValueError(f"lse must be fp32 [{rows}, {hq}], contiguous, on the pages' device")
-        shape = (lens.shape[0], heads, table.shape[-1])
-        if out is None:
-            out = torch.empty(shape, dtype=torch.float32, device=q.device)
-        else:
-            if (out.shape != shape or out.dtype != torch.float32 or not out.is_contiguous()
-                    or out.get_device() != self._dev):
-                raise ValueError(f"out must be fp32 {list(shape)}, contiguous, on the pages' device")
-        args = (hq, self.head_dim ** -0.5 if scale is None else scale, window)
-        need = self._C.paged_block_mass_workspace(pg, batch, qa, args)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        self._call(self._C.paged_block_mass, pg, batch, qa, lse.data_ptr(), out.data_ptr(), args,
-                   ws.data_ptr() if need else 0, need)
-        return out
+        return self._ops.block_mass(q, lse, table, lens, starts, scale, window, max_new, out)
