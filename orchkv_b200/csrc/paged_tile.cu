@@ -31,7 +31,11 @@ __device__ int g_paged_dead;
 
 constexpr int kThreads = 384;
 constexpr uint32_t kR = 256, kK = 128;
+// Columns of tensor memory: the weights of half 0, the scores, the weights of
+// half 1 (64, 128 and 64 columns), then O of either half.
+constexpr uint32_t kP0 = 0, kS = 64, kP1 = 192;
 constexpr float kGrow = 8.f;               // log2 of the growth that O is scaled at
+constexpr int kPolyEvery = 99;              // every fourth pair of powers goes to the FMA units
 constexpr int kMeta = 8;                   // tiles whose column masks are kept
 
 template <int DP> struct TileCfg {
@@ -42,7 +46,7 @@ template <int DP> struct TileCfg {
 };
 
 struct TileShared {
-    ull full[8], empty[8], s_full[2], p_full[2], q_full[2], o_full[2], fix, drain;
+    ull full[8], empty[8], s_full[2], p_full[2], q_full[2], o_full[2], s_free, fix, drain;
     uint32_t tmem;
     int dead;
     alignas(16) uint32_t mask[kMeta][4];   // columns of a tile that hold a token
@@ -80,6 +84,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             mbar_init(smem_addr(&sh.q_full[k]), 4);
             mbar_init(smem_addr(&sh.o_full[k]), 1);
         }
+        mbar_init(smem_addr(&sh.s_free), 4);
         mbar_init(smem_addr(&sh.fix), 1);
         mbar_init(smem_addr(&sh.drain), 1);
         sh.dead = 0;
@@ -95,12 +100,20 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
     // 4 x 88 + 8 x 208 registers a lane are the 12 x 168 of the launch
     if (wid < 4) {
       regs_down<88>();
-      if (wid == 0) {
-        // ---- loads ----
+      if (wid == 0 || wid == 2) {
+        // ---- loads: K by one warp, V by another, into every other place of the ring ----
+        const bool is_v = wid == 2;
+        const CUtensorMap *map = is_v ? &vmap : &kmap;
         const uint32_t bs = p.bs.d, per = bs < kK ? kK / bs : 1, box = bs < kK ? bs : kK;
+        const uint32_t page_bytes = box * 128, all_pages = per == 32 ? 0xFFFFFFFFu : (1u << per) - 1;
         constexpr uint32_t halves = DP / 64;
-        uint32_t st = 0, ph = 0, fix_ph = 0, tile_no = 0, issued = 0;
+        uint32_t st = is_v ? 1 : 0, ph = 0, fix_ph = 0, tile_no = 0;
+        const bool one = elect_one();
         bool ok = true;
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+            if (ok) ok = mbar_wait(bar, parity, dead);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+        };
         do {
             const uint32_t h = w.at.h, i = w.at.i;
             const int zh = by_head ? 0 : (int)h;
@@ -111,144 +124,167 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 return page_of(b, p.n_pages, i, h, k0 / p.bs);
             };
             int pg = page(w.t0);
-            for (uint32_t t = w.t0; ok && t < w.t1; t++) {
+            for (uint32_t t = w.t0; ok && t < w.t1; t++, tile_no++) {
                 const uint32_t k0 = (w.first + t) * kK;
                 const int nxt = page(t + 1);
                 const uint32_t have = __ballot_sync(0xFFFFFFFFu, pg >= 0);
-                // column masks of the tile, one word a lane
-                uint32_t word = 0;
-                const uint32_t c0 = (lane & 3) * 32;
-                for (uint32_t q = c0 / bs; q * bs < c0 + 32 && q < per; q++)
-                    if (have >> q & 1) {
-                        const uint32_t lo = max(q * bs, c0) - c0;
-                        const uint32_t hi = min((bs < kK ? (q + 1) * bs : kK), c0 + 32) - c0;
-                        word |= (hi == 32 ? 0xFFFFFFFFu : (1u << hi) - 1) & ~((1u << lo) - 1);
-                    }
-                const int lim = w.s.len - (int)(k0 + c0);
-                if (lim <= 0) word = 0;
-                else if (lim < 32) word &= (1u << lim) - 1;
-                const bool part = __any_sync(0xFFFFFFFFu, word != 0xFFFFFFFFu);
-                const uint32_t bytes = __popc(have) * box * 128 * halves;
-                const int y = bs < kK ? 0 : (int)(k0 % bs);
-#pragma unroll 1
-                for (int kv = 0; ok && kv < 2; kv++) {
-                    ok = mbar_wait(smem_addr(&sh.empty[st]), ph ^ 1, dead);
-                    ok = __all_sync(0xFFFFFFFFu, ok);
-                    if (!ok) break;
-                    if (kv == 0 && lane < 4) sh.mask[tile_no % kMeta][lane] = word;
-                    const uint32_t full = smem_addr(&sh.full[st]);
-                    const bool fix = kv == 1 && part;
-                    const uint32_t bar = fix ? smem_addr(&sh.fix) : full;
-                    const uint32_t dst = ring + st * Cfg::tile;
-                    __syncwarp();
-                    if (lane == 0) mbar_expect(bar, bytes);
-                    __syncwarp();
-                    if (pg >= 0)
+                // columns that hold a token, one word a lane
+                const bool part = have != all_pages || (int)(k0 + kK) > w.s.len;
+                uint32_t word = 0xFFFFFFFFu;
+                if (part) {
+                    word = 0;
+                    const uint32_t c0 = (lane & 3) * 32;
+                    for (uint32_t q = c0 / p.bs; q * bs < c0 + 32 && q < per; q++)
+                        if (have >> q & 1) {
+                            const uint32_t lo = max(q * bs, c0) - c0;
+                            const uint32_t hi = min((bs < kK ? (q + 1) * bs : kK), c0 + 32) - c0;
+                            word |= (hi == 32 ? 0xFFFFFFFFu : (1u << hi) - 1) & ~((1u << lo) - 1);
+                        }
+                    const int lim = w.s.len - (int)(k0 + c0);
+                    if (lim <= 0) word = 0;
+                    else if (lim < 32) word &= (1u << lim) - 1;
+                }
+                const uint32_t full = smem_addr(&sh.full[st]), dst = ring + st * Cfg::tile;
+                const bool fix = is_v && part;
+                const uint32_t bar = fix ? smem_addr(&sh.fix) : full;
+                wait(smem_addr(&sh.empty[st]), ph ^ 1);
+                if (!ok) break;
+                if (!is_v && lane < 4) sh.mask[tile_no % kMeta][lane] = word;
+                __syncwarp();
+                if (one) mbar_expect(bar, __popc(have) * page_bytes * halves);
+                __syncwarp();
+                const int y = bs < kK ? 0 : (int)(k0 - k0 / p.bs * bs);
+                // one thread, one page after another: a warp whose lanes issue
+                // copies of their own takes four times as long for each
+                for (uint32_t q = 0; q < per; q++) {
+                    const int pq = __shfl_sync(0xFFFFFFFFu, pg, q);
+                    if (one && pq >= 0)
 #pragma unroll
                         for (uint32_t x = 0; x < halves; x++)
-                            tma4(dst + x * kK * 128 + lane * box * 128, kv ? &vmap : &kmap, (int)x * 64, y, zh,
-                                 pg, bar);
-                    if (fix) {
-                        // rows of V without a token become zeros: their weights
-                        // are 0, and 0 times a stale NaN would not be
-                        ok = mbar_wait(bar, fix_ph, dead);
-                        ok = __all_sync(0xFFFFFFFFu, ok);
-                        fix_ph ^= 1;
-                        for (uint32_t r = lane; r < kK; r += 32) {
-                            const uint32_t wd = __shfl_sync(0xFFFFFFFFu, word, r >> 5);
-                            if (!(wd >> (r & 31) & 1))
-#pragma unroll
-                                for (uint32_t x = 0; x < halves; x++)
-#pragma unroll
-                                    for (uint32_t c = 0; c < 8; c++)
-                                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
-                                                         dst + x * kK * 128 + r * 128 + c * 16), "r"(0) : "memory");
-                        }
-                        fence_async();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(full);
-                    }
-                    issued++;
-                    if (++st == ST) { st = 0; ph ^= 1; }
+                            tma4(dst + x * kK * 128 + q * page_bytes, map, (int)x * 64, y, zh, pq, bar);
                 }
+                __syncwarp();
+                if (fix) {
+                    // rows of V without a token become zeros: their weights are
+                    // 0, and 0 times a stale NaN would not be
+                    wait(bar, fix_ph);
+                    fix_ph ^= 1;
+                    for (uint32_t r = lane; r < kK; r += 32) {
+                        const uint32_t wd = __shfl_sync(0xFFFFFFFFu, word, r >> 5);
+                        if (!(wd >> (r & 31) & 1))
+#pragma unroll
+                            for (uint32_t x = 0; x < halves; x++)
+#pragma unroll
+                                for (uint32_t c = 0; c < 8; c++)
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                                                     dst + x * kK * 128 + r * 128 + c * 16), "r"(0) : "memory");
+                    }
+                    fence_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full);
+                }
+                st += 2;
+                if (st >= ST) { st -= ST; ph ^= 1; }
                 pg = nxt;
-                tile_no++;
             }
         } while (ok && w.next());
         if (!ok) {
             // leave no copy in flight behind
             if (lane == 0)
-                for (uint32_t k = 0; k < ST && k < issued; k++) {
-                    st = st == 0 ? ST - 1 : st - 1;
-                    if (st == ST - 1) ph ^= 1;
+                for (uint32_t k = 0; k < (ST + 1) / 2 && k < tile_no; k++) {
+                    if (st < 2) { st += ST; ph ^= 1; }
+                    st -= 2;
                     mbar_drain(smem_addr(&sh.full[st]), ph);
                 }
             __syncwarp();
         }
       } else if (wid == 1) {
         // ---- products ----
-        if (lane == 0) {
-            const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-            const uint32_t id_qk = inst_desc(f, 128, kK, 0), id_pv = inst_desc(f, 128, DP, 1);
-            uint32_t st = 0, ph = 0, q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
-            bool ok = true;
-            auto qk = [&](int x, uint32_t stage) {
-                const uint32_t qa = q_s + x * 128 * DP * 2, ka = ring + stage * Cfg::tile;
+        const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+        const uint32_t id_qk = inst_desc(f, 128, kK, 0), id_pv = inst_desc(f, 128, DP, 1);
+        const uint32_t q_lo = desc_lo(q_s, 16), k_lo = desc_lo(ring, 16), v_lo = desc_lo(ring, kK * 128);
+        uint32_t st = 0, ph = 0, q_ph[2] = {0, 0}, p_ph[2] = {0, 0}, s_no = 0;
+        bool ok = true;
+        const bool one = elect_one();
+        auto wait = [&](ull &bar, uint32_t parity) {
+            if (ok) ok = mbar_wait(smem_addr(&bar), parity, dead);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+        };
+        // scores of half x into the one buffer, once its last ones are read
+        auto qk = [&](int x, uint32_t stage) {
+            wait(sh.s_free, (s_no & 1) ^ 1);
+            s_no++;
+            if (!ok) return;
+            tm_after();
+            if (one) {
+                const uint32_t qa = q_lo + x * (128 * DP * 2 >> 4), ka = k_lo + stage * (Cfg::tile >> 4);
 #pragma unroll
                 for (int k = 0; k < DP / 16; k++) {
-                    const uint32_t o = (k >> 2) * kK * 128 + (k & 3) * 32;
-                    mma_ss(tm + x * 128, smem_desc(qa + o, 16, 1024), smem_desc(ka + o, 16, 1024), id_qk, k > 0);
+                    const uint32_t o = ((k >> 2) * kK * 128 + (k & 3) * 32) >> 4;
+                    mma_ss(tm + kS, qa + o, ka + o, id_qk, k > 0);
                 }
                 tm_commit(smem_addr(&sh.s_full[x]));
-            };
-            do {
-                const int nx = w.live() > 128 ? 2 : 1;
-                uint32_t ks = st;
-                ok = mbar_wait(smem_addr(&sh.full[ks]), ph, dead);
-                if (!ok) break;
-                for (int x = 0; ok && x < nx; x++) {
-                    ok = mbar_wait(smem_addr(&sh.q_full[x]), q_ph[x], dead);
-                    q_ph[x] ^= 1;
-                    tm_after();
-                    if (ok) qk(x, ks);
-                }
-                if (!ok) break;
-                tm_commit(smem_addr(&sh.empty[ks]));
+            }
+            __syncwarp();
+        };
+        auto release = [&](uint32_t stage) {
+            if (one) tm_commit(smem_addr(&sh.empty[stage]));
+            __syncwarp();
+        };
+        do {
+            const int nx = w.live() > 128 ? 2 : 1;
+            uint32_t ks = st;
+            wait(sh.full[ks], ph);
+            for (int x = 0; ok && x < nx; x++) {
+                wait(sh.q_full[x], q_ph[x]);
+                q_ph[x] ^= 1;
+                if (ok) qk(x, ks);
+            }
+            if (!ok) break;
+            release(ks);
+            if (++st == ST) { st = 0; ph ^= 1; }
+            for (uint32_t t = w.t0; ok && t < w.t1; t++) {
+                const bool more = t + 1 < w.t1;
+                const uint32_t vs = st;
+                wait(sh.full[vs], ph);
                 if (++st == ST) { st = 0; ph ^= 1; }
-                for (uint32_t t = w.t0; ok && t < w.t1; t++) {
-                    const bool more = t + 1 < w.t1;
-                    const uint32_t vs = st;
-                    ok = mbar_wait(smem_addr(&sh.full[vs]), ph, dead);
+                if (more) {
+                    ks = st;
+                    wait(sh.full[ks], ph);
                     if (++st == ST) { st = 0; ph ^= 1; }
-                    if (ok && more) {
-                        ks = st;
-                        ok = mbar_wait(smem_addr(&sh.full[ks]), ph, dead);
-                        if (++st == ST) { st = 0; ph ^= 1; }
-                    }
-                    for (int x = 0; ok && x < nx; x++) {
-                        ok = mbar_wait(smem_addr(&sh.p_full[x]), p_ph[x], dead);
-                        p_ph[x] ^= 1;
-                        if (!ok) break;
-                        tm_after();
-                        const uint32_t va = ring + vs * Cfg::tile;
+                }
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    if (!ok || x >= nx) break;
+                    // the next scores first: their half reads them as soon as
+                    // its weights are out
+                    if (more) qk(x, ks);
+                    wait(sh.p_full[x], p_ph[x]);
+                    p_ph[x] ^= 1;
+                    if (!ok) break;
+                    tm_after();
+                    if (one) {
+                        const uint32_t va = v_lo + vs * (Cfg::tile >> 4);
 #pragma unroll
                         for (int k = 0; k < kK / 16; k++)
-                            mma_ts(tm + 256 + x * 128, tm + x * 128 + k * 8,
-                                   smem_desc(va + k * 2048, kK * 128, 1024), id_pv, t > w.t0 || k > 0);
-                        if (more) qk(x, ks);
-                        else tm_commit(smem_addr(&sh.o_full[x]));
+                            mma_ts(tm + 256 + x * 128, tm + (x ? kP1 : kP0) + k * 8, va + k * (2048 >> 4), id_pv,
+                                   k > 0 || t > w.t0);
+                        tm_commit(smem_addr(&sh.o_full[x]));
                     }
-                    if (!ok) break;
-                    tm_commit(smem_addr(&sh.empty[vs]));
-                    if (more) tm_commit(smem_addr(&sh.empty[ks]));
+                    __syncwarp();
                 }
-            } while (ok && w.next());
-            if (!ok) {
+                if (!ok) break;
+                release(vs);
+                if (more) release(ks);
+            }
+        } while (ok && w.next());
+        if (!ok) {
+            if (one) {
                 tm_commit(smem_addr(&sh.drain));
                 mbar_drain(smem_addr(&sh.drain), 0);
             }
+            __syncwarp();
         }
-        __syncwarp();
       }
     } else {
         regs_up<208>();
@@ -256,7 +292,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         const int x = (wid - 4) >> 2;
         const uint32_t r = threadIdx.x - 128 - x * 128;    // row of the half
         const uint32_t lanes = (wid & 3) << 21;            // first lane of this warp, in a TMEM address
-        const uint32_t S = tm + x * 128 + lanes, O = tm + 256 + x * 128 + lanes;
+        const uint32_t S = tm + kS + lanes, P = tm + (x ? kP1 : kP0) + lanes, O = tm + 256 + x * 128 + lanes;
         uint32_t s_ph = 0, o_ph = 0, tile_no = 0;
         const ull sl2 = f2(a.sl2, a.sl2);
 
@@ -301,9 +337,14 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
 #pragma unroll
                 for (int c = 0; c < 4; c++) tm_ld32(S + c * 32, s + c * 32);
                 tm_wait_ld();
+                tm_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&sh.s_free));
                 const int k0 = (int)((w.first + t) * kK);
                 const uint4 mk = *(const uint4 *)sh.mask[tile_no % kMeta];
-                if (k0 < all_lo || k0 + (int)kK - 1 > all_hi || (mk.x & mk.y & mk.z & mk.w) != 0xFFFFFFFFu) {
+                const bool masked = k0 < all_lo || k0 + (int)kK - 1 > all_hi ||
+                                    (mk.x & mk.y & mk.z & mk.w) != 0xFFFFFFFFu;
+                if (masked) {
                     const uint32_t mw[4] = {mk.x, mk.y, mk.z, mk.w};
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
@@ -316,16 +357,24 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                             if (!(bits >> j & 1)) s[c * 32 + j] = -INFINITY;
                     }
                 }
-                float mx[4] = {s[0], s[1], s[2], s[3]};
+                float mx[4];
 #pragma unroll
-                for (int j = 4; j < 128; j += 4)
+                for (int k = 0; k < 4; k++) mx[k] = fmaxf(s[k], s[k + 4]);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) mx[k] = fmaxf(mx[k], s[j + k]);
+                for (int j = 8; j < 128; j += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) mx[k] = max3(mx[k], s[j + k], s[j + k + 4]);
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 const float ms = top * a.sl2;          // the scale is positive here
                 if (t == w.t0) {
                     m = ms;
                 } else {
+                    // the last product has read P and written O
+                    ok = mbar_wait(smem_addr(&sh.o_full[x]), o_ph, dead);
+                    ok = __all_sync(0xFFFFFFFFu, ok);
+                    if (!ok) break;
+                    o_ph ^= 1;
+                    tm_after();
                     const bool grow = ms > m + kGrow || (m == -INFINITY && ms > m);
                     if (__any_sync(0xFFFFFFFFu, grow)) {
                         const float nm = grow ? ms : m;
@@ -351,21 +400,31 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 // weights: rounded to the pages' type for the product (half a
                 // step each, as the result's own rounding); their sum is taken
                 // before that
+                auto weigh = [&](auto poly) {
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t pk[16];
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t pk[16];
 #pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        float *e = s + c * 32 + 2 * j;
-                        float u, v;
-                        unf2(fma2(f2(e[0], e[1]), sl2, nm2), &u, &v);
-                        u = ex2(u);
-                        v = ex2(v);
-                        l2[j & 1] = add2(l2[j & 1], f2(u, v));
-                        pk[j] = pack2<T>(u, v);
+                        for (int j = 0; j < 16; j++) {
+                            const float *e = s + c * 32 + 2 * j;
+                            const ull z = fma2(f2(e[0], e[1]), sl2, nm2);
+                            float u, v;
+                            if (decltype(poly)::value && j % kPolyEvery == kPolyEvery - 1) {
+                                unf2(ex2_poly<4>(z), &u, &v);
+                            } else {
+                                unf2(z, &u, &v);
+                                u = ex2(u);
+                                v = ex2(v);
+                            }
+                            l2[j & 1] = add2(l2[j & 1], f2(u, v));
+                            pk[j] = pack2<T>(u, v);
+                        }
+                        tm_st16(P + c * 16, pk);
                     }
-                    tm_st16(S + c * 16, pk);
-                }
+                };
+                // (a masked score's power has to be 0, not the polynomial's 2^-126)
+                if (masked) weigh(std::false_type());
+                else weigh(std::true_type());
                 tm_wait_st();
                 tm_before();
                 __syncwarp();
@@ -755,42 +814,54 @@ mass_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         }
       } else if (wid == 1) {
         // ---- products ----
-        if (lane == 0) {
-            const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-            const uint32_t id = inst_desc(f, 128, 128, 0);
-            uint32_t u_no = 0, st = 0, ph = 0, tile = 0;
-            bool ok = true;
-            do {
-                const uint32_t kb = u_no & 1;
-                ok = mbar_wait(smem_addr(&sh.k_full[kb]), u_no >> 1 & 1, dead);
-                for (uint32_t t = w.t0; ok && t < w.t1; t++, tile++) {
-                    ok = mbar_wait(smem_addr(&sh.q_full[st]), ph, dead);
-                    for (int x = 0; ok && x < 2; x++) {
-                        const uint32_t sb = x * 2 + (tile & 1);
-                        ok = mbar_wait(smem_addr(&sh.s_empty[sb]), (tile >> 1 & 1) ^ 1, dead);
-                        if (!ok) break;
-                        tm_after();
-                        const uint32_t ka = keys_s + (kb * 2 + x) * Cfg::tile, qa = ring + st * Cfg::tile;
+        const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+        const uint32_t id = inst_desc(f, 128, 128, 0);
+        const uint32_t k_lo = desc_lo(keys_s, 16), q_lo = desc_lo(ring, 16);
+        uint32_t u_no = 0, st = 0, ph = 0, tile = 0;
+        bool ok = true;
+        const bool one = elect_one();
+        auto wait = [&](ull &bar, uint32_t parity) {
+            if (ok) ok = mbar_wait(smem_addr(&bar), parity, dead);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+        };
+        do {
+            const uint32_t kb = u_no & 1;
+            wait(sh.k_full[kb], u_no >> 1 & 1);
+            for (uint32_t t = w.t0; ok && t < w.t1; t++, tile++) {
+                wait(sh.q_full[st], ph);
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const uint32_t sb = x * 2 + (tile & 1);
+                    wait(sh.s_empty[sb], (tile >> 1 & 1) ^ 1);
+                    if (!ok) break;
+                    tm_after();
+                    if (one) {
+                        const uint32_t ka = k_lo + (kb * 2 + x) * (Cfg::tile >> 4), qa = q_lo + st * (Cfg::tile >> 4);
 #pragma unroll
                         for (int k = 0; k < DP / 16; k++) {
-                            const uint32_t o = (k >> 2) * 128 * 128 + (k & 3) * 32;
-                            mma_ss(tm + sb * 128, smem_desc(ka + o, 16, 1024), smem_desc(qa + o, 16, 1024), id, k > 0);
+                            const uint32_t o = ((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4;
+                            mma_ss(tm + sb * 128, ka + o, qa + o, id, k > 0);
                         }
                         tm_commit(smem_addr(&sh.s_full[sb]));
                     }
-                    if (!ok) break;
-                    tm_commit(smem_addr(&sh.q_empty[st]));
-                    if (++st == RQ) { st = 0; ph ^= 1; }
+                    __syncwarp();
                 }
-                if (ok) tm_commit(smem_addr(&sh.k_empty[kb]));
-                u_no++;
-            } while (ok && w.next());
-            if (!ok) {
+                if (!ok) break;
+                if (one) tm_commit(smem_addr(&sh.q_empty[st]));
+                __syncwarp();
+                if (++st == RQ) { st = 0; ph ^= 1; }
+            }
+            if (ok && one) tm_commit(smem_addr(&sh.k_empty[kb]));
+            __syncwarp();
+            u_no++;
+        } while (ok && w.next());
+        if (!ok) {
+            if (one) {
                 tm_commit(smem_addr(&sh.drain));
                 mbar_drain(smem_addr(&sh.drain), 0);
             }
+            __syncwarp();
         }
-        __syncwarp();
       } else if (wid == 2) {
         // ---- the rows' lse ----
         uint32_t st = 0, ph = 0;

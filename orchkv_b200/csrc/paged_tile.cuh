@@ -138,32 +138,41 @@ __device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t *r)
         : "memory");
 }
 
-// Shared-memory operand, 128-byte swizzle: start address, byte strides.  For
-// an operand whose k runs along the 128-byte rows, sbo is the distance of
-// 8-row groups (lbo unused); for one whose m or n runs along them, lbo is the
-// distance of 64-element column groups and sbo that of 8-row (k) groups.
-__device__ __forceinline__ ull smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo)
-{
-    return (ull)((addr & 0x3FFFF) >> 4) | (ull)(lbo >> 4) << 16 | (ull)(sbo >> 4) << 32 | 1ull << 46 |
-           2ull << 61;
-}
+// Shared-memory operand, 128-byte swizzle: start address and byte strides.  For
+// an operand whose k runs along the 128-byte rows, 8-row groups are 1024 bytes
+// apart; for one whose n runs along them, `lbo` is the distance of its
+// 64-element column groups and 8-row (k) groups are 1024 bytes apart.  The low
+// word varies (addresses stay below 2^18: no carry), the high one is kDescHi.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return addr >> 4 | (lbo >> 4) << 16; }
+constexpr uint32_t kDescHi = 1024 >> 4 | 1u << 14 | 2u << 29;
 // kind::f16, fp32 sums: fmt 0 fp16, 1 bf16 (both operands); b_mn: B's n runs
 // along its rows.
 __host__ __device__ constexpr uint32_t inst_desc(uint32_t fmt, uint32_t M, uint32_t N, uint32_t b_mn)
 {
     return 1u << 4 | fmt << 7 | fmt << 10 | b_mn << 16 | (N >> 3) << 17 | (M >> 4) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, ull a, ull b, uint32_t id, bool add)
+// One thread of a warp issues; every operand is the same for the whole warp.
+// A single thread's instructions are what limits the rate of products, so the
+// descriptors are one 32-bit add each.
+__device__ __forceinline__ bool elect_one()
 {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(id), "r"((uint32_t)add) : "memory");
+    uint32_t y;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(y));
+    return y != 0;
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, ull b, uint32_t id, bool add)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, bool add)
 {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(id), "r"((uint32_t)add) : "memory");
+    asm volatile("{\n.reg .pred p;\n.reg .b64 a, b;\nsetp.ne.u32 p, %4, 0;\n"
+                 "mov.b64 a, {%1, %5};\nmov.b64 b, {%2, %5};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(id), "r"((uint32_t)add), "n"(kDescHi) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, bool add)
+{
+    asm volatile("{\n.reg .pred p;\n.reg .b64 b;\nsetp.ne.u32 p, %4, 0;\n"
+                 "mov.b64 b, {%2, %5};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(id), "r"((uint32_t)add), "n"(kDescHi) : "memory");
 }
 
 // ---- pairs of fp32 ---------------------------------------------------------------------
@@ -234,6 +243,13 @@ __device__ __forceinline__ void tma3(uint32_t dst, const CUtensorMap *map, int x
                  "[%0], [%1, {%3, %4, %5}], [%2];"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
