@@ -273,8 +273,8 @@ __host__ __device__ inline size_t slot_floats(uint32_t R, uint32_t D) { return (
 
 // The slots of the pieces of the unit that boundary c (at position `at`, offset
 // `off` of its sequence) is the first to cut, in key order: slot 2(c-1)+1 for
-// the unit's start, held by CTA c - 1, then 2c, 2(c+1), ...; ~0 for an empty
-// piece.  A thread takes a boundary.  Returns their number (at most kMaxPieces).
+// the unit's start, held by CTA c - 1, then 2c, 2(c+1), ... but for empty
+// pieces.  A thread takes a boundary.  Returns their number.
 constexpr uint32_t kMaxPieces = 600;
 template <int NT, class Where>
 __device__ uint32_t find_pieces(const BatchDev &b, uint32_t c, uint32_t C, const Pos &at, ull off, ull share,
@@ -282,7 +282,8 @@ __device__ uint32_t find_pieces(const BatchDev &b, uint32_t c, uint32_t C, const
 {
     constexpr uint32_t kOut = 0xFFFFFFFFu;
     __shared__ uint32_t t_s[NT + 1];
-    __shared__ uint32_t n_s;
+    __shared__ uint32_t n_w[NT / 32];
+    const uint32_t lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         t_s[0] = at.t;
         slots[0] = 2 * (c - 1) + 1;
@@ -299,19 +300,25 @@ __device__ uint32_t find_pieces(const BatchDev &b, uint32_t c, uint32_t C, const
         t_s[threadIdx.x + 1] = t;
         __syncthreads();
         const uint32_t from = t_s[threadIdx.x], to = t == kOut ? nt : t;
-        if (from != kOut && cc < C && 1 + k0 + threadIdx.x < kMaxPieces) {
-            slots[1 + k0 + threadIdx.x] = to > from ? 2 * cc : kOut;
-            if (t == kOut) n_s = 2 + k0 + threadIdx.x;     // the last one
-        }
+        const bool piece = from != kOut && cc < C && to > from;
+        const uint32_t in = __ballot_sync(0xFFFFFFFFu, piece);
+        if (lane == 0) n_w[wid] = __popc(in);
         const bool more = t_s[NT] != kOut;
         __syncthreads();
+        uint32_t before = n;
+#pragma unroll
+        for (int k = 0; k < NT / 32; k++) {
+            if (k < (int)wid) before += n_w[k];
+            n += n_w[k];
+        }
+        before += __popc(in & ((1u << lane) - 1));
+        if (piece && before < kMaxPieces) slots[before] = 2 * cc;
         if (!more) break;
         if (threadIdx.x == 0) t_s[0] = t_s[NT];
         __syncthreads();
-        n += NT;
     }
     __syncthreads();
-    return min(n_s, kMaxPieces);
+    return min(n, kMaxPieces);
 }
 
 // The pieces of every cut unit into its rows.  Block c looks at boundary c: it
@@ -349,21 +356,36 @@ join_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint32_t pa
     for (uint32_t e = part * each * d4 + threadIdx.x; e < r_end * d4; e += NT) {
         const uint32_t rr = e / d4, d = (e - rr * d4) * 4;
         float M = -INFINITY, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (uint32_t k = 0; k < K; k++) {
-            if (slots[k] == 0xFFFFFFFFu) continue;
-            const float *sl = slot_of(sp.ws, slots[k], R, D);
-            const float m = sl[rr], l = sl[R + rr];
-            const float4 v = *(const float4 *)(sl + 2 * R + (size_t)rr * D + d);
-            const float nm = fmaxf(M, m), ms = nm == -INFINITY ? 0.f : nm;
-            const float f = exp2f(M - ms), w = exp2f(m - ms);
+        for (uint32_t k0 = 0; k0 < K; k0 += 8) {           // eight pieces' loads at once
+            float m[8], l[8];
+            float4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const bool in = k0 + k < K;
+                const float *sl = slot_of(sp.ws, slots[in ? k0 + k : 0], R, D);
+                m[k] = in ? sl[rr] : -INFINITY;
+                l[k] = sl[R + rr];
+                v[k] = *(const float4 *)(sl + 2 * R + (size_t)rr * D + d);
+            }
+            float nm = M;
+#pragma unroll
+            for (int k = 0; k < 8; k++) nm = fmaxf(nm, m[k]);
+            const float ms = nm == -INFINITY ? 0.f : nm, f = exp2f(M - ms);
             M = nm;
-            L = L * f + w * l;
-            // a piece without an attended token holds zeros
-            o[0] = o[0] * f + w * v.x;
-            o[1] = o[1] * f + w * v.y;
-            o[2] = o[2] * f + w * v.z;
-            o[3] = o[3] * f + w * v.w;
+            L *= f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[j] *= f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                // a piece without an attended token holds zeros, one past the
+                // last weighs nothing
+                const float w = exp2f(m[k] - ms);
+                L += k0 + k < K ? w * l[k] : 0.f;
+                o[0] += k0 + k < K ? w * v[k].x : 0.f;
+                o[1] += k0 + k < K ? w * v[k].y : 0.f;
+                o[2] += k0 + k < K ? w * v[k].z : 0.f;
+                o[3] += k0 + k < K ? w * v[k].w : 0.f;
+            }
         }
         const float Ms = M == -INFINITY ? 0.f : M;
         const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;

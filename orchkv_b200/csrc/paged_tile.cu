@@ -1032,7 +1032,7 @@ mass_join_kernel(MassGeo g, PagesDev p, BatchDev b, MassDev a, SplitDev sp)
     float y = 0.f;
 #pragma unroll 4
     for (uint32_t k = 0; k < K; k++)
-        if (slots[k] != 0xFFFFFFFFu) y += sp.ws[(size_t)slots[k] * kMassSlot + lb];
+        y += sp.ws[(size_t)slots[k] * kMassSlot + lb];
     a.mass[((size_t)at.i * g.H + at.h) * b.width + gb] = y;
 }
 
