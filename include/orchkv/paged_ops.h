@@ -49,7 +49,8 @@ typedef struct orchkv_pages {
  * table[i * table_seq_stride + h * table_head_stride + t / page_tokens];
  * entries outside [0, n_pages) name no page.  starts must not decrease; rows
  * from starts[n_seqs] on belong to no sequence and are left alone.  max_new
- * is an upper bound of one sequence's new tokens (rows if unknown). */
+ * is an upper bound of one sequence's new tokens (n_rows if unknown); the rows
+ * of a sequence that has more may not be computed. */
 typedef struct orchkv_batch {
     const int32_t *table;
     int64_t  table_seq_stride, table_head_stride;   /* head stride 0: one table for all heads */

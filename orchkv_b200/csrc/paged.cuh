@@ -204,8 +204,10 @@ struct ClassDev {
     uint32_t min_rows, max_rows;
 };
 // ctas: persistent CTAs that divide the work; ws: 2 * ctas partial slots.
+// split: instead, each unit (tiles_max row tiles a sequence and KV head) is a
+// cluster of so many CTAs.
 struct SplitDev {
-    uint32_t ctas;
+    uint32_t ctas, split, tiles_max;
     float *ws;
 };
 constexpr uint32_t kSimtRows = 8, kSimtKeys = 128;
@@ -216,7 +218,8 @@ int launch_mass_simt(const PagesDev &p, const BatchDev &b, const MassDev &a,
                      const ClassDev &cl, cudaStream_t s);
 
 constexpr uint32_t kRowsRows = 16;
-uint32_t attend_rows_ctas(uint32_t D, unsigned long long units, unsigned long long keys);
+SplitDev attend_rows_split(uint32_t D, uint32_t n, uint32_t H, uint32_t tiles_max, unsigned long long units,
+                           unsigned long long keys);
 int launch_attend_rows(int dtype, const PagesDev &p, const BatchDev &b, const AttendDev &a,
                        const ClassDev &cl, const SplitDev &sp, cudaStream_t s);
 int launch_mass_rows(int dtype, const PagesDev &p, const BatchDev &b, const MassDev &a,

@@ -101,8 +101,12 @@ AttendPlan plan_attend(const orchkv_pages_t *p, const orchkv_batch_t *b, const o
     if (tile) units = std::min(units, H * b->n_seqs * (kFewRows / R));
     pl.few = ClassDev{0, tile ? kFewRows : 0xFFFFFFFFu};
     pl.many = ClassDev{kFewRows, 0xFFFFFFFFu};
-    pl.rows.ctas = p->dtype == DTYPE_FP32 ? attend_simt_ctas(units, keys)
-                                          : attend_rows_ctas(p->d_head, units, keys);
+    if (p->dtype == DTYPE_FP32)
+        pl.rows.ctas = attend_simt_ctas(units, keys);
+    else
+        pl.rows = attend_rows_split(p->d_head, b->n_seqs, p->n_kv_heads,
+                                    std::max<uint32_t>(1, (std::min<uint64_t>(most, pl.few.max_rows) + R - 1) / R),
+                                    units, keys);
     if (tile) pl.tile.ctas = attend_tile_ctas(H * (b->n_rows * G / kTileRows + b->n_seqs), keys);
     // both may use the same memory: the tile kernel starts when the rows are joined
     const size_t row = (p->d_head + 2) * sizeof(float) * 2;
@@ -189,7 +193,7 @@ int orchkv_paged_attend(const orchkv_pages_t *pages, const orchkv_batch_t *batch
     const size_t e = dtype_size((DataType)pages->dtype);
     if (!rows_ok(args->q, e) || !rows_ok(args->out, e)) return ORCHKV_ERR_INVALID;
     AttendPlan pl = plan_attend(pages, batch, args);
-    if (!workspace || (uintptr_t)workspace % 256 || bytes < pl.bytes) return ORCHKV_ERR_INVALID;
+    if (pl.bytes && (!workspace || (uintptr_t)workspace % 256 || bytes < pl.bytes)) return ORCHKV_ERR_INVALID;
     AttendDev a;
     a.q = rows_dev(args->q, e);
     a.out = rows_dev(args->out, e);

@@ -32,9 +32,36 @@ template <int DP> struct RowsCfg {
     static constexpr size_t smem = kW * ring;
 };
 
-template <class T, int DP>
+// One value of another CTA of the cluster's shared memory, at the address that
+// `p` has in this one.
+__device__ __forceinline__ float4 peer4(const float *p, uint32_t rank)
+{
+    uint32_t a;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float peer1(const float *p, uint32_t rank)
+{
+    uint32_t a;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void cluster_meet()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// CL: a unit is one cluster of `split` CTAs, which share its keys equally and
+// join their parts over each other's shared memory; else the CTAs share the
+// whole call's work and join_kernel adds cut units.
+template <class T, int DP, bool CL>
 __global__ void __launch_bounds__(kW * 32, RowsCfg<DP>::ctas)
-attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp)
+attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint32_t split, uint32_t tiles_max)
 {
     using Cfg = RowsCfg<DP>;
     constexpr int ST = Cfg::stages;
@@ -47,11 +74,20 @@ attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp)
     const uint32_t ring_a = smem_addr(ring);
 
     Pos at, end;
-    ull W;
-    find_share<kW * 32>(g, b, p.bs.d, blockIdx.x, sp.ctas, &sh, &at, &end, &W);
-    // the join behind this launch may be scheduled now; it waits for our end
-    cudaTriggerProgrammaticLaunchCompletion();
-    if (W == 0) return;
+    uint32_t rank = 0;
+    if (CL) {
+        const uint32_t u = blockIdx.x / split, ih = u / tiles_max;
+        rank = blockIdx.x - u * split;
+        at = Pos{ih / g.H, ih % g.H, u - ih * tiles_max, 0};
+        end = Pos{b.n, 0, 0, 0};
+        if (at.rt >= row_tiles(g, load_seq(b, p.bs.d, at.i))) return;   // the whole cluster
+    } else {
+        ull W;
+        find_share<kW * 32>(g, b, p.bs.d, blockIdx.x, sp.ctas, &sh, &at, &end, &W);
+        // the join behind this launch may be scheduled now; it waits for our end
+        cudaTriggerProgrammaticLaunchCompletion();
+        if (W == 0) return;
+    }
     while (at.i < b.n) {
         const SeqDev s = load_seq(b, p.bs.d, at.i);
         const uint32_t RT = row_tiles(g, s);
@@ -60,8 +96,9 @@ attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp)
         if (stop && end.t == 0) break;
         uint32_t first, nt;
         key_tiles(g, s, at.rt, &first, &nt);
-        const uint32_t t0 = at.t, t1 = stop ? end.t : nt;
-        if (t0 < t1) {
+        const uint32_t t0 = CL ? rank * nt / split : at.t;
+        const uint32_t t1 = CL ? (rank + 1) * nt / split : stop ? end.t : nt;
+        if (CL || t0 < t1) {
             const uint32_t rows = (uint32_t)s.m * g.G, pr0 = at.rt * kR;
             const RowInfo r0 = row_info(g, s, at.h, pr0 + (lane >> 2));
             const RowInfo r1 = row_info(g, s, at.h, pr0 + (lane >> 2) + 8);
@@ -196,8 +233,9 @@ attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp)
                         make_float2(acc[n][2 * x], acc[n][2 * x + 1]);
             }
             __syncthreads();
-            const bool whole = t0 == 0 && t1 == nt;
-            float *sl = whole ? nullptr : slot_of(sp.ws, 2 * blockIdx.x + (t0 == 0 ? 1 : 0), kR, D);
+            const bool whole = CL ? split == 1 : t0 == 0 && t1 == nt;
+            // (a cluster's parts lie as a slot does)
+            float *sl = CL ? (float *)(smem + Cfg::smem) : whole ? nullptr : slot_of(sp.ws, 2 * blockIdx.x + (t0 == 0 ? 1 : 0), kR, D);
             const uint32_t live = min(kR, rows - pr0), d8 = D / 8;
             for (uint32_t e = threadIdx.x; e < live * d8; e += kW * 32) {
                 const uint32_t r = e / d8, d = (e - r * d8) * 8;
@@ -229,6 +267,51 @@ attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp)
                         a.lse[(size_t)ri.row * a.Hq + ri.head] =
                             L > 0.f ? (Ms + log2f(L)) * kLn2 : L == 0.f ? -INFINITY : L;
                 }
+            }
+            if (CL) {
+                if (!whole) {
+                    cluster_meet();
+                    const uint32_t d4 = D / 4;
+                    for (uint32_t e = rank * (kW * 32) + threadIdx.x; e < live * d4; e += split * (kW * 32)) {
+                        const uint32_t r = e / d4, d = (e - r * d4) * 4;
+                        float M = -INFINITY, L = 0.f, o[4] = {};
+#pragma unroll 1
+                        for (uint32_t k0 = 0; k0 < split; k0 += 4) {
+                            float m[4], l[4];
+                            float4 v[4];
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const uint32_t c = min(k0 + k, split - 1);
+                                m[k] = peer1(sl + r, c);
+                                l[k] = peer1(sl + kR + r, c);
+                                v[k] = peer4(sl + 2 * kR + r * D + d, c);
+                            }
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                if (k0 + k >= split) break;
+                                const float nm = fmaxf(M, m[k]), ms = nm == -INFINITY ? 0.f : nm;
+                                const float f = ex2(M - ms), w = ex2(m[k] - ms);
+                                M = nm;
+                                L = L * f + w * l[k];
+                                o[0] = o[0] * f + w * v[k].x;
+                                o[1] = o[1] * f + w * v[k].y;
+                                o[2] = o[2] * f + w * v[k].z;
+                                o[3] = o[3] * f + w * v[k].w;
+                            }
+                        }
+                        const RowInfo ri = row_info(g, s, at.h, pr0 + r);
+                        const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+                        *(uint2 *)(a.out.p + (long long)ri.row * a.out.row_b + (long long)ri.head * a.out.head_b +
+                                   d * 2) = make_uint2(pack2<T>(o[0] * inv, o[1] * inv),
+                                                       pack2<T>(o[2] * inv, o[3] * inv));
+                        if (a.lse && d == 0)
+                            a.lse[(size_t)ri.row * a.Hq + ri.head] =
+                                L > 0.f ? ((M == -INFINITY ? 0.f : M) + log2f(L)) * kLn2
+                                        : L == 0.f ? -INFINITY : L;
+                    }
+                    cluster_meet();                    // nobody leaves while its part is read
+                }
+                return;
             }
             __syncthreads();
         }
@@ -387,15 +470,48 @@ mass_rows_kernel(Geo g, PagesDev p, BatchDev b, MassDev a, uint32_t per_item, ui
     for (uint32_t k = lane; k < n_blk; k += 32) out[k] = mass_s[wid][k];
 }
 
+// CTAs of a unit's cluster, 0: the equal shares.  A cluster needs no join
+// launch (5 us of a call), but its CTAs are one unit's for the whole launch;
+// so it is taken when the units and their splits are one wave of two CTAs an
+// SM, or need none, and no CTA has more than 8 key tiles to do.
+uint32_t cluster_split(unsigned long long units, unsigned long long keys)
+{
+    const unsigned long long tiles = (keys + kKeys - 1) / kKeys;
+    uint32_t s = 1;
+    while (s < 16 && s < tiles && units * s * 2 <= 148 * 2) s *= 2;
+    return tiles <= 8ull * s && units * s < (1u << 30) ? s : 0;
+}
+
 template <class T, int DP>
 int attend_d(const PagesDev &p, const BatchDev &b, const AttendDev &a, const ClassDev &cl,
              const SplitDev &sp, cudaStream_t s)
 {
     const Geo g = {kR, kKeys, a.G, p.H, a.window, cl.min_rows, cl.max_rows};
-    auto k = attend_rows_kernel<T, DP>;
+    if (sp.split) {
+        auto k = attend_rows_kernel<T, DP, true>;
+        constexpr size_t smem = RowsCfg<DP>::smem + (size_t)kR * (DP + 2) * sizeof(float);
+        static std::atomic<uint64_t> done, wide;
+        OKV_CUDA_TRY(allow_smem(k, smem, done));
+        if (sp.split > 8) OKV_CUDA_TRY(allow_wide_cluster(k, wide));
+        cudaLaunchConfig_t c = {};
+        c.gridDim = dim3(b.n * p.H * sp.tiles_max * sp.split);
+        c.blockDim = dim3(kW * 32);
+        c.dynamicSmemBytes = smem;
+        c.stream = s;
+        cudaLaunchAttribute at;
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = sp.split;
+        at.val.clusterDim.y = at.val.clusterDim.z = 1;
+        c.attrs = &at;
+        c.numAttrs = 1;
+        OKV_CUDA_TRY(cudaLaunchKernelEx(&c, k, g, p, b, a, sp, sp.split, sp.tiles_max));
+        note_launches(1);
+        return ORCHKV_OK;
+    }
+    auto k = attend_rows_kernel<T, DP, false>;
     static std::atomic<uint64_t> done;
     OKV_CUDA_TRY(allow_smem(k, RowsCfg<DP>::smem, done));
-    k<<<sp.ctas, kW * 32, RowsCfg<DP>::smem, s>>>(g, p, b, a, sp);
+    k<<<sp.ctas, kW * 32, RowsCfg<DP>::smem, s>>>(g, p, b, a, sp, 1, 1);
     note_launches(1);
     OKV_CUDA_TRY(cudaGetLastError());
     if (sp.ctas > 1) {
@@ -432,11 +548,17 @@ int mass_d(const PagesDev &p, const BatchDev &b, const MassDev &a, const ClassDe
 
 }  // namespace
 
-uint32_t attend_rows_ctas(uint32_t D, unsigned long long units, unsigned long long keys)
+SplitDev attend_rows_split(uint32_t D, uint32_t n, uint32_t H, uint32_t tiles_max, unsigned long long units,
+                           unsigned long long keys)
 {
+    SplitDev sp = {};
+    sp.tiles_max = tiles_max;
+    sp.split = cluster_split((unsigned long long)n * H * tiles_max, keys);
+    if (sp.split) return sp;
     const unsigned long long tiles = units * ((keys + kKeys - 1) / kKeys);
     const unsigned long long most = 148ull * (D > 128 ? 1 : 2);
-    return (uint32_t)(tiles < most ? tiles : most);
+    sp.ctas = (uint32_t)(tiles < most ? tiles : most);
+    return sp;
 }
 
 int launch_attend_rows(int dtype, const PagesDev &p, const BatchDev &b, const AttendDev &a,

@@ -413,6 +413,17 @@ template <class K> cudaError_t allow_smem(K k, size_t bytes, std::atomic<uint64_
     return e;
 }
 
+// Clusters of more than 8 CTAs, once a kernel and device.
+template <class K> cudaError_t allow_wide_cluster(K k, std::atomic<uint64_t> &done)
+{
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && done.load() >> dev & 1)) return e;
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && dev < 64) done |= 1ull << dev;
+    return e;
+}
+
 // A launch that may begin before the one in front of it in the stream has
 // ended (the kernel waits itself with cudaGridDependencySynchronize).
 template <class... P, class... A>

@@ -194,7 +194,8 @@ class PagedKV:
         Returns out, or (out, lse) with lse [rows, query heads] fp32.  A row
         with nothing to attend to gets 0 and -inf.  max_new: the most new
         tokens of one sequence, if the caller knows it (decode: 1), lets the
-        call leave out what only longer ones need."""
+        call leave out what only longer ones need; the rows of a sequence
+        with more of them may not be computed."""
         return self._ops.attend(q, table, lens, starts, scale, window, max_new, return_lse, out)
 
     def block_mass(self, q, lse, table, lens, starts, *, scale: float | None = None, window: int = 0,

@@ -17,7 +17,7 @@ A = 1 << 20                                       # any aligned address: never r
 def call(**kw):
     """A valid call's arguments, by name, with some replaced."""
     v = dict(k=A, v=A, page_stride=16 * 4 * 128, head_stride=128, token_stride=4 * 128, n_pages=9,
-             page_tokens=16, n_kv_heads=4, d_head=128, dtype=1, table=A, width=8, n=2, lens=A, starts=A,
+             page_tokens=16, n_kv_heads=4, d_head=128, dtype=1, table=A, width=4096, n=2, lens=A, starts=A,
              rows=6, hq=8, q=A, out=A, row_stride=8 * 128, q_head=128, kr=A, vr=A, rot=128, turns=A,
              ws=A, short=0)
     assert set(kw) <= set(v)
@@ -70,6 +70,7 @@ def test_nothing_to_do():
         assert fn["append"]() == 0 and fn["attend"]() == 0
     assert call(n=0, table=0, lens=0, starts=0)[1]["mass"]() == 0
     assert call()[0] > 0
+    assert call(width=4, rows=2)[0] == 0          # short: no workspace
     assert call(d_head=100)[0] == 0
 
 
