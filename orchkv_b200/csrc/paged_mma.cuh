@@ -110,6 +110,33 @@ __device__ __forceinline__ void load_rows16(uint32_t dst, const char *base, long
     }
 }
 
+// The same when the 16 rows lie in one page, tok_b apart from `off` on (the
+// whole warp's; negative: no page); rows outside `have` become zeros.
+template <int DP>
+__device__ __forceinline__ void load_run16(uint32_t dst, const char *base, long long off, long long tok_b,
+                                           uint32_t have, uint32_t D)
+{
+    const uint32_t lane = threadIdx.x & 31;
+    constexpr int LPR = DP / 8, RPI = 32 / LPR;
+    const uint32_t r0 = lane / LPR, c = lane % LPR;
+    const bool col = c * 8 < D;
+    const char *src = base + (have ? off : 0) + c * 16 + r0 * tok_b;
+#pragma unroll
+    for (int j = 0; j < 16 / RPI; j++) {
+        const uint32_t r = j * RPI + r0;
+        const bool ok = col && (have >> r & 1);
+        cp16(dst + swz<DP>(r, c), ok ? src : base, ok);
+        src += RPI * tok_b;
+    }
+}
+// Bits [lo, hi] of 16.
+__device__ __forceinline__ uint32_t bits16(int lo, int hi)
+{
+    lo = lo < 0 ? 0 : lo;
+    hi = hi > 15 ? 15 : hi;
+    return hi < lo ? 0u : ((2u << hi) - 1) & ~((1u << lo) - 1);
+}
+
 // s[2][4] = scores of 16 keys (tiles of 8) against the 16 rows.
 template <class T, int DP>
 __device__ __forceinline__ void scores16(uint32_t kt, const uint32_t (*qf)[4], float (*s)[4])

@@ -59,7 +59,8 @@ __device__ __forceinline__ void cluster_meet()
 // CL: a unit is one cluster of `split` CTAs, which share its keys equally and
 // join their parts over each other's shared memory; else the CTAs share the
 // whole call's work and join_kernel adds cut units.
-template <class T, int DP, bool CL>
+// AL: pages of whole 16-key groups, so a group's rows lie side by side.
+template <class T, int DP, bool CL, bool AL>
 __global__ void __launch_bounds__(kW * 32, RowsCfg<DP>::ctas)
 attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint32_t split, uint32_t tiles_max)
 {
@@ -110,11 +111,14 @@ attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint
             uint32_t qf[DP / 16][4];
             load_q_frag<T, DP>(a.q, r0, r1, D, qf);
 
-            // page of this lane's key (lanes 0..15) of group t, one group ahead
-            auto key_of = [&](uint32_t t) { return (int)((first + t) * kKeys + wid * 16 + (lane & 15)); };
+            // page of this lane's key (lanes 0..15; AL: of the group) of group t,
+            // one group ahead
+            auto key_of = [&](uint32_t t) {
+                return (int)((first + t) * kKeys + wid * 16 + (AL ? 0 : (lane & 15)));
+            };
             auto page = [&](uint32_t t) {
                 const int key = key_of(t);
-                if (t >= t1 || key < any_lo || key > any_hi) return -1;
+                if (t >= t1 || key + (AL ? 15 : 0) < any_lo || key > any_hi) return -1;
                 return page_of(b, p.n_pages, at.i, at.h, (uint32_t)key / p.bs);
             };
             auto issue = [&](uint32_t t, int pg, uint32_t st) {
@@ -124,11 +128,17 @@ attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint
                     if (pg >= 0)
                         off = pg * p.page_b + at.h * p.head_b +
                               (long long)((uint32_t)key - (uint32_t)key / p.bs * p.bs.d) * p.tok_b;
-                    const uint32_t have = __ballot_sync(0xFFFFFFFFu, pg >= 0) & 0xFFFFu;
+                    const uint32_t have = AL ? (pg >= 0 ? bits16(any_lo - key, any_hi - key) : 0u)
+                                             : __ballot_sync(0xFFFFFFFFu, pg >= 0) & 0xFFFFu;
                     if (lane == 0) have_s[wid][st] = have;
                     const uint32_t kt = ring_a + st * 2 * Cfg::tile;
-                    load_rows16<DP>(kt, p.k, off, D);
-                    load_rows16<DP>(kt + Cfg::tile, p.v, off, D);
+                    if (AL) {
+                        load_run16<DP>(kt, p.k, off, p.tok_b, have, D);
+                        load_run16<DP>(kt + Cfg::tile, p.v, off, p.tok_b, have, D);
+                    } else {
+                        load_rows16<DP>(kt, p.k, off, D);
+                        load_rows16<DP>(kt + Cfg::tile, p.v, off, D);
+                    }
                 }
                 cp_commit();
             };
@@ -334,6 +344,125 @@ attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint
 constexpr int kMassStages = 6;
 constexpr uint32_t kMaxRun = 64;                       // blocks of a warp's run
 
+// Pages of whole 16-key groups: a group lies in one block, so its 16 x 16
+// weights add up to one number; a thread keeps its share of a block until the
+// block ends.
+template <class T, int DP>
+__global__ void __launch_bounds__(kW * 32)
+mass_runs_kernel(Geo g, PagesDev p, BatchDev b, MassDev a, uint32_t run, uint32_t groups)
+{
+    constexpr int ST = kMassStages;
+    constexpr uint32_t tile = 16 * DP * 2;
+    extern __shared__ __align__(128) char smem[];
+    __shared__ float mass_s[kW][kMaxRun];
+    const uint32_t lane = threadIdx.x & 31, wid = threadIdx.x >> 5, D = p.D;
+    const uint32_t ring_a = smem_addr(smem + wid * ST * tile);
+    const uint32_t x = blockIdx.x % groups, ih = blockIdx.x / groups;
+    const uint32_t h = ih % p.H, i = ih / p.H;
+    const SeqDev s = load_seq(b, p.bs.d, i);
+    const uint32_t rows = (uint32_t)s.m * g.G;
+    if ((rows <= g.min_rows && g.min_rows) || rows > g.max_rows) return;
+
+    const uint32_t b0 = (x * kW + wid) * run;
+    if (b0 >= b.width) return;
+    const uint32_t n_blk = min(run, b.width - b0), per = p.bs.d / 16;    // groups of a block
+    for (uint32_t k = lane; k < n_blk; k += 32) mass_s[wid][k] = 0.f;
+    __syncwarp();
+    const int key0 = (int)(b0 * p.bs.d);
+
+    for (uint32_t rt = 0; rt * kR < rows; rt++) {
+        const RowInfo r0 = row_info(g, s, h, rt * kR + (lane >> 2));
+        const RowInfo r1 = row_info(g, s, h, rt * kR + (lane >> 2) + 8);
+        const RowInfo rf = row_info(g, s, h, rt * kR);
+        const RowInfo rl = row_info(g, s, h, min((rt + 1) * kR, rows) - 1);
+        const int any_lo = rf.lo, any_hi = rl.hi, all_lo = rl.lo, all_hi = rf.hi;
+        // the blocks of the run that hold a key of this row tile
+        if (any_hi < key0 || any_lo >= key0 + (int)(n_blk * p.bs.d)) continue;
+        const uint32_t first = any_lo > key0 ? (uint32_t)(any_lo - key0) / p.bs : 0;
+        const uint32_t last = min((uint32_t)(any_hi - key0) / p.bs, n_blk - 1);
+
+        uint32_t qf[DP / 16][4];
+        load_q_frag<T, DP>(a.q, r0, r1, D, qf);
+        // a row behind the last weighs nothing
+        float ls[2];
+        ls[0] = r0.row >= 0 ? a.lse[(size_t)r0.row * a.Hq + r0.head] * kLog2e : INFINITY;
+        ls[1] = r1.row >= 0 ? a.lse[(size_t)r1.row * a.Hq + r1.head] * kLog2e : INFINITY;
+
+        // the next group to load (block, group in it, page) and to weigh
+        uint32_t lb = first, lg = 0, wb = first, wg = 0;
+        auto page = [&](uint32_t blk) { return blk <= last ? page_of(b, p.n_pages, i, h, b0 + blk) : -1; };
+        int pg = page(lb), pg_next = page(lb + 1);
+        auto have_of = [&](uint32_t blk, uint32_t gr) {
+            const int k = key0 + (int)(blk * p.bs.d + gr * 16);
+            return bits16(any_lo - k, any_hi - k);
+        };
+        auto issue = [&](uint32_t st) {
+            if (lb <= last) {
+                const uint32_t have = pg >= 0 ? have_of(lb, lg) : 0;
+                if (have)
+                    load_run16<DP>(ring_a + st * tile, p.k,
+                                   pg * p.page_b + h * p.head_b + (long long)(lg * 16) * p.tok_b, p.tok_b, have, D);
+                if (++lg == per) {
+                    lg = 0;
+                    lb++;
+                    pg = pg_next;
+                    pg_next = page(lb + 1);
+                }
+            }
+            cp_commit();
+        };
+#pragma unroll
+        for (int k = 0; k < ST - 1; k++) issue(k);
+        uint32_t st = 0, st_in = ST - 1;
+        int pw = page(first), pw_next = page(first + 1);   // of the block being weighed
+        float part = 0.f;
+        while (wb <= last) {
+            issue(st_in);
+            st_in = st_in + 1 == ST ? 0 : st_in + 1;
+            cp_wait<ST - 1>();
+            __syncwarp();
+            const uint32_t have = pw >= 0 ? have_of(wb, wg) : 0, kt = ring_a + st * tile;
+            st = st + 1 == ST ? 0 : st + 1;
+            if (have) {
+                const int k0 = key0 + (int)(wb * p.bs.d + wg * 16);
+                float sc[2][4];
+                scores16<T, DP>(kt, qf, sc);
+                if (have == 0xFFFFu && k0 >= all_lo && k0 + 15 <= all_hi) {
+                    float e[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) e[j] = ex2(sc[j >> 2][j & 3] * a.sl2 - ls[j >> 1 & 1]);
+                    part += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const uint32_t col = (j >> 2) * 8 + (lane & 3) * 2 + (j & 1);
+                        const RowInfo &r = j & 2 ? r1 : r0;
+                        const int key = k0 + (int)col;
+                        if ((have >> col & 1) && key <= r.hi && key >= r.lo)
+                            part += ex2(sc[j >> 2][j & 3] * a.sl2 - ls[j >> 1 & 1]);
+                    }
+                }
+            }
+            if (++wg == per) {
+#pragma unroll
+                for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xFFFFFFFFu, part, o);
+                if (lane == 0) mass_s[wid][wb] += part;
+                part = 0.f;
+                wg = 0;
+                wb++;
+                pw = pw_next;
+                pw_next = page(wb + 1);
+            }
+            __syncwarp();
+        }
+        cp_wait<0>();
+        __syncwarp();
+    }
+    __syncwarp();
+    float *out = a.mass + ((size_t)i * p.H + h) * b.width + b0;
+    for (uint32_t k = lane; k < n_blk; k += 32) out[k] = mass_s[wid][k];
+}
+
 template <class T, int DP>
 __global__ void __launch_bounds__(kW * 32)
 mass_rows_kernel(Geo g, PagesDev p, BatchDev b, MassDev a, uint32_t per_item, uint32_t items_per_warp,
@@ -473,22 +602,24 @@ mass_rows_kernel(Geo g, PagesDev p, BatchDev b, MassDev a, uint32_t per_item, ui
 // CTAs of a unit's cluster, 0: the equal shares.  A cluster needs no join
 // launch (5 us of a call), but its CTAs are one unit's for the whole launch;
 // so it is taken when the units and their splits are one wave of two CTAs an
-// SM, or need none, and no CTA has more than 8 key tiles to do.
+// SM, or need none, and no CTA has more than 8 key tiles to do.  A CTA gets two
+// tiles at least (one request over 900 tokens: 8.2 us with 8 CTAs a unit, 9.5
+// with 15).
 uint32_t cluster_split(unsigned long long units, unsigned long long keys)
 {
     const unsigned long long tiles = (keys + kKeys - 1) / kKeys;
     uint32_t s = 1;
-    while (s < 16 && s < tiles && units * s * 2 <= 148 * 2) s *= 2;
+    while (s < 16 && 2 * s < tiles && units * s * 2 <= 148 * 2) s *= 2;
     return tiles <= 8ull * s && units * s < (1u << 30) ? s : 0;
 }
 
-template <class T, int DP>
-int attend_d(const PagesDev &p, const BatchDev &b, const AttendDev &a, const ClassDev &cl,
+template <class T, int DP, bool AL>
+int attend_a(const PagesDev &p, const BatchDev &b, const AttendDev &a, const ClassDev &cl,
              const SplitDev &sp, cudaStream_t s)
 {
     const Geo g = {kR, kKeys, a.G, p.H, a.window, cl.min_rows, cl.max_rows};
     if (sp.split) {
-        auto k = attend_rows_kernel<T, DP, true>;
+        auto k = attend_rows_kernel<T, DP, true, AL>;
         constexpr size_t smem = RowsCfg<DP>::smem + (size_t)kR * (DP + 2) * sizeof(float);
         static std::atomic<uint64_t> done, wide;
         OKV_CUDA_TRY(allow_smem(k, smem, done));
@@ -508,7 +639,7 @@ int attend_d(const PagesDev &p, const BatchDev &b, const AttendDev &a, const Cla
         note_launches(1);
         return ORCHKV_OK;
     }
-    auto k = attend_rows_kernel<T, DP, false>;
+    auto k = attend_rows_kernel<T, DP, false, AL>;
     static std::atomic<uint64_t> done;
     OKV_CUDA_TRY(allow_smem(k, RowsCfg<DP>::smem, done));
     k<<<sp.ctas, kW * 32, RowsCfg<DP>::smem, s>>>(g, p, b, a, sp, 1, 1);
@@ -519,6 +650,13 @@ int attend_d(const PagesDev &p, const BatchDev &b, const AttendDev &a, const Cla
         note_launches(1);
     }
     return ORCHKV_OK;
+}
+
+template <class T, int DP>
+int attend_d(const PagesDev &p, const BatchDev &b, const AttendDev &a, const ClassDev &cl,
+             const SplitDev &sp, cudaStream_t s)
+{
+    return p.bs.d % 16 == 0 ? attend_a<T, DP, true>(p, b, a, cl, sp, s) : attend_a<T, DP, false>(p, b, a, cl, sp, s);
 }
 
 template <class T, int DP>
@@ -536,11 +674,17 @@ int mass_d(const PagesDev &p, const BatchDev &b, const MassDev &a, const ClassDe
     const uint32_t groups = (items + run * kW - 1) / (run * kW);
     const unsigned long long grid = (unsigned long long)b.n * p.H * groups;
     if (grid > 0x7FFFFFFFull) return ORCHKV_ERR_INVALID;
-    auto k = mass_rows_kernel<T, DP>;
     const size_t smem = (size_t)kW * kMassStages * 16 * DP * 2;
-    static std::atomic<uint64_t> done;
-    OKV_CUDA_TRY(allow_smem(k, smem, done));
-    k<<<(unsigned)grid, kW * 32, smem, s>>>(g, p, b, a, per_item, run, groups);
+    static std::atomic<uint64_t> done, done_al;
+    if (p.bs.d % 16 == 0) {
+        auto k = mass_runs_kernel<T, DP>;
+        OKV_CUDA_TRY(allow_smem(k, smem, done_al));
+        k<<<(unsigned)grid, kW * 32, smem, s>>>(g, p, b, a, run, groups);
+    } else {
+        auto k = mass_rows_kernel<T, DP>;
+        OKV_CUDA_TRY(allow_smem(k, smem, done));
+        k<<<(unsigned)grid, kW * 32, smem, s>>>(g, p, b, a, per_item, run, groups);
+    }
     note_launches(1);
     OKV_CUDA_TRY(cudaGetLastError());
     return ORCHKV_OK;
