@@ -13,6 +13,8 @@
 // loads).  The warps' parts are joined in shared memory once a unit, the
 // CTAs' as paged_split.cuh describes.  Places outside the range of every row,
 // past the length or in no page are filled with zeros and never read.
+#include <algorithm>
+
 #include "kernels.h"
 #include "paged_mma.cuh"
 
@@ -112,7 +114,7 @@ attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint
             load_q_frag<T, DP>(a.q, r0, r1, D, qf);
 
             // page of this lane's key (lanes 0..15; AL: of the group) of group t,
-            // one group ahead
+            // asked for one group ahead
             auto key_of = [&](uint32_t t) {
                 return (int)((first + t) * kKeys + wid * 16 + (AL ? 0 : (lane & 15)));
             };
@@ -341,7 +343,7 @@ attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint
 // column sums of exp(s - lse) over the 16 rows are three shuffles.  The masses
 // of the run stay in shared memory over the row tiles, so each is written
 // once, in one order of sums.
-constexpr int kMassStages = 6;
+constexpr int kMassStages = 3;
 constexpr uint32_t kMaxRun = 64;                       // blocks of a warp's run
 
 // Pages of whole 16-key groups: a group lies in one block, so its 16 x 16
@@ -388,10 +390,17 @@ mass_runs_kernel(Geo g, PagesDev p, BatchDev b, MassDev a, uint32_t run, uint32_
         ls[0] = r0.row >= 0 ? a.lse[(size_t)r0.row * a.Hq + r0.head] * kLog2e : INFINITY;
         ls[1] = r1.row >= 0 ? a.lse[(size_t)r1.row * a.Hq + r1.head] * kLog2e : INFINITY;
 
-        // the next group to load (block, group in it, page) and to weigh
+        // the next group to load (block, group in it) and to weigh; a lane
+        // holds the pages of two blocks of the run (of at most 64)
         uint32_t lb = first, lg = 0, wb = first, wg = 0;
         auto page = [&](uint32_t blk) { return blk <= last ? page_of(b, p.n_pages, i, h, b0 + blk) : -1; };
-        int pg = page(lb), pg_next = page(lb + 1);
+        const int pa = page(first + lane), pb = page(first + 32 + lane);
+        auto page_at = [&](uint32_t blk) {
+            const uint32_t k = blk - first;
+            const int x = __shfl_sync(0xFFFFFFFFu, pa, k & 31), y = __shfl_sync(0xFFFFFFFFu, pb, k & 31);
+            return k < 32 ? x : y;
+        };
+        int pg = page_at(first);
         auto have_of = [&](uint32_t blk, uint32_t gr) {
             const int k = key0 + (int)(blk * p.bs.d + gr * 16);
             return bits16(any_lo - k, any_hi - k);
@@ -405,8 +414,7 @@ mass_runs_kernel(Geo g, PagesDev p, BatchDev b, MassDev a, uint32_t run, uint32_
                 if (++lg == per) {
                     lg = 0;
                     lb++;
-                    pg = pg_next;
-                    pg_next = page(lb + 1);
+                    pg = page_at(min(lb, last));
                 }
             }
             cp_commit();
@@ -414,7 +422,7 @@ mass_runs_kernel(Geo g, PagesDev p, BatchDev b, MassDev a, uint32_t run, uint32_
 #pragma unroll
         for (int k = 0; k < ST - 1; k++) issue(k);
         uint32_t st = 0, st_in = ST - 1;
-        int pw = page(first), pw_next = page(first + 1);   // of the block being weighed
+        int pw = page_at(first);                           // of the block being weighed
         float part = 0.f;
         while (wb <= last) {
             issue(st_in);
@@ -450,8 +458,7 @@ mass_runs_kernel(Geo g, PagesDev p, BatchDev b, MassDev a, uint32_t run, uint32_
                 part = 0.f;
                 wg = 0;
                 wb++;
-                pw = pw_next;
-                pw_next = page(wb + 1);
+                pw = page_at(min(wb, last));
             }
             __syncwarp();
         }
@@ -665,12 +672,15 @@ int mass_d(const PagesDev &p, const BatchDev &b, const MassDev &a, const ClassDe
     const Geo g = {kR, 0, a.G, p.H, a.window, cl.min_rows, cl.max_rows};
     const uint32_t per_item = p.bs.d >= 16 ? 1 : 16 / p.bs.d;
     const uint32_t items = (b.width + per_item - 1) / per_item;
-    // run length: enough warps for about 8 an SM and CTA slot, runs as long as
-    // that leaves (a run pays its first loads' latency once)
-    const unsigned long long all = (unsigned long long)b.n * p.H * items;
-    uint32_t run = (uint32_t)(all / (148ull * 3 * kW * 2));
+    // A CTA takes 4 us to its first product (rows, queries, table, keys one
+    // after the other), as long as 30 blocks take: as few and as long runs as
+    // leave no place (3 an SM) of the device empty.  32 requests over 8192
+    // tokens: 101 us with 16 CTAs a place, 77 with 8, 61 with 4.
     const uint32_t most = kMaxRun / per_item;
-    run = run < 1 ? 1 : run > most ? most : run;
+    unsigned long long groups64 = 148ull * 3 / ((unsigned long long)b.n * p.H);
+    groups64 = std::max<unsigned long long>(groups64, (items + most * kW - 1) / (most * kW));
+    groups64 = std::max<unsigned long long>(groups64, 1);
+    const uint32_t run = (uint32_t)((items + groups64 * kW - 1) / (groups64 * kW));
     const uint32_t groups = (items + run * kW - 1) / (run * kW);
     const unsigned long long grid = (unsigned long long)b.n * p.H * groups;
     if (grid > 0x7FFFFFFFull) return ORCHKV_ERR_INVALID;
