@@ -35,7 +35,6 @@ constexpr uint32_t kR = 256, kK = 128;
 // half 1 (64, 128 and 64 columns), then O of either half.
 constexpr uint32_t kP0 = 0, kS = 64, kP1 = 192;
 constexpr float kGrow = 8.f;               // log2 of the growth that O is scaled at
-constexpr int kPolyEvery = 99;              // every fourth pair of powers goes to the FMA units
 constexpr int kMeta = 8;                   // tiles whose column masks are kept
 
 template <int DP> struct TileCfg {
@@ -400,31 +399,21 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 // weights: rounded to the pages' type for the product (half a
                 // step each, as the result's own rounding); their sum is taken
                 // before that
-                auto weigh = [&](auto poly) {
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        uint32_t pk[16];
+                for (int c = 0; c < 4; c++) {
+                    uint32_t pk[16];
 #pragma unroll
-                        for (int j = 0; j < 16; j++) {
-                            const float *e = s + c * 32 + 2 * j;
-                            const ull z = fma2(f2(e[0], e[1]), sl2, nm2);
-                            float u, v;
-                            if (decltype(poly)::value && j % kPolyEvery == kPolyEvery - 1) {
-                                unf2(ex2_poly<4>(z), &u, &v);
-                            } else {
-                                unf2(z, &u, &v);
-                                u = ex2(u);
-                                v = ex2(v);
-                            }
-                            l2[j & 1] = add2(l2[j & 1], f2(u, v));
-                            pk[j] = pack2<T>(u, v);
-                        }
-                        tm_st16(P + c * 16, pk);
+                    for (int j = 0; j < 16; j++) {
+                        const float *e = s + c * 32 + 2 * j;
+                        float u, v;
+                        unf2(fma2(f2(e[0], e[1]), sl2, nm2), &u, &v);
+                        u = ex2(u);
+                        v = ex2(v);
+                        l2[j & 1] = add2(l2[j & 1], f2(u, v));
+                        pk[j] = pack2<T>(u, v);
                     }
-                };
-                // (a masked score's power has to be 0, not the polynomial's 2^-126)
-                if (masked) weigh(std::false_type());
-                else weigh(std::true_type());
+                    tm_st16(P + c * 16, pk);
+                }
                 tm_wait_st();
                 tm_before();
                 __syncwarp();
@@ -533,7 +522,8 @@ int go(const CUtensorMap &km, const CUtensorMap &vm, const PagesDev &p, const Ba
 // buffers a group.  CTAs cut the list of units as the attention does; pieces
 // of one unit are added by mass_join_kernel in row order.
 
-constexpr int kMassThreads = 384;
+constexpr int kMassThreads = 640;
+constexpr int kMassPoly = 2;                           // of 8 pairs of powers, those on the FMA units
 constexpr uint32_t kMK = 256;                          // keys of a unit
 
 constexpr int kMassRing = 3;                           // query tiles
@@ -668,7 +658,7 @@ struct MassShared {
     ull k_full[2], k_empty[2], q_full[kMassRing], q_empty[kMassRing], s_full[4], s_empty[4], drain, sums[3];
     uint32_t tmem;
     int dead;
-    alignas(16) float lse[kMassRing][128];                     // of a query tile's rows, times log2(e)
+    alignas(16) float lse[kMassRing][128];                     // of a query tile's rows, times -log2(e)
     alignas(16) float key[kMK];
     SplitShared split;
 };
@@ -725,7 +715,7 @@ mass_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             mbar_init(smem_addr(&sh.q_full[k]), 2);
             mbar_init(smem_addr(&sh.q_empty[k]), 9);
         }
-        for (int k = 0; k < 3; k++) mbar_init(smem_addr(&sh.sums[k]), k < 2 ? 4 : 8);
+        for (int k = 0; k < 3; k++) mbar_init(smem_addr(&sh.sums[k]), k < 2 ? 8 : 16);
         for (int k = 0; k < 4; k++) {
             mbar_init(smem_addr(&sh.s_full[k]), 1);
             mbar_init(smem_addr(&sh.s_empty[k]), 4);
@@ -742,6 +732,7 @@ mass_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                          ring + st * Cfg::tile + x * 128 * 128 + row * 128 + c * 16), "r"(0) : "memory");
     }
     for (uint32_t e = threadIdx.x; e < RQ * 128; e += kMassThreads) sh.lse[e >> 7][e & 127] = 0.f;
+    for (uint32_t e = threadIdx.x; e < kMK; e += kMassThreads) sh.key[e] = 0.f;
     fence_async();
     if (wid == 1) tm_alloc(smem_addr(&sh.tmem), 512);
     tm_before();
@@ -751,7 +742,6 @@ mass_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     volatile int *dead = &sh.dead;
 
     if (wid < 4) {
-      regs_down<88>();
       if (wid == 0) {
         // ---- loads ----
         const uint32_t bs = p.bs.d, per = bs < 128 ? 128 / bs : 1, box = bs < 128 ? bs : 128;
@@ -873,9 +863,9 @@ mass_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                 for (int k = 0; k < 4; k++) {
                     const uint32_t c = lane + 32 * k, j = c / g.G;
                     const int tok = w.a + (int)(t * g.toks + j);
-                    v[k] = c < cols ? 0.f : INFINITY;  // a column of no row weighs nothing
+                    v[k] = c < cols ? 0.f : -INFINITY; // a column of no row weighs nothing
                     if (c < cols && tok < w.e)
-                        v[k] = a.lse[(size_t)(w.s.start + tok) * a.Hq + w.at.h * g.G + (c - j * g.G)] * kLog2e;
+                        v[k] = a.lse[(size_t)(w.s.start + tok) * a.Hq + w.at.h * g.G + (c - j * g.G)] * -kLog2e;
                 }
                 ok = mbar_wait(smem_addr(&sh.q_empty[st]), ph ^ 1, dead);
                 ok = __all_sync(0xFFFFFFFFu, ok);
@@ -889,12 +879,12 @@ mass_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         } while (ok && w.next());
       }
     } else {
-        regs_up<208>();
-        // ---- sums of one half's keys ----
-        const int x = (wid - 4) >> 2;
-        const uint32_t r = threadIdx.x - 128 - x * 128;
+        // ---- sums of one half's keys, over every other query tile ----
+        const int x = (wid - 4) >> 2 & 1;
+        const uint32_t y = (wid - 4) >> 3;                 // the tiles of this parity
+        const uint32_t r = (threadIdx.x - 128) & 127;
         const uint32_t lanes = (wid & 3) << 21;
-        const ull sl2 = f2(a.sl2, a.sl2), neg = f2(-1.f, -1.f);
+        const ull sl2 = f2(a.sl2, a.sl2);
         uint32_t st = 0, ph = 0, tile = 0, sum_ph = 0;
         bool ok = true, live = true;
         while (live && ok) {
@@ -907,7 +897,11 @@ mass_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             if (g.window) je = min(je, key - w.s.c0 + (int)g.window);
             ull sum[2] = {0, 0};
             for (uint32_t t = w.t0; t < w.t1; t++, tile++) {
-                const uint32_t sb = x * 2 + (tile & 1);
+                if ((tile & 1) != y) {
+                    if (++st == RQ) { st = 0; ph ^= 1; }
+                    continue;
+                }
+                const uint32_t sb = x * 2 + y;
                 ok = mbar_wait(smem_addr(&sh.s_full[sb]), tile >> 1 & 1, dead) &&
                      mbar_wait(smem_addr(&sh.q_full[st]), ph, dead);
                 ok = __all_sync(0xFFFFFFFFu, ok);
@@ -935,12 +929,18 @@ mass_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 #pragma unroll
                         for (int j = 0; j < 8; j++) {
                             const float4 l4 = ls[j];
-                            const ull u = fma2(f2(s[4 * j], s[4 * j + 1]), sl2, mul2(f2(l4.x, l4.y), neg));
-                            const ull v = fma2(f2(s[4 * j + 2], s[4 * j + 3]), sl2, mul2(f2(l4.z, l4.w), neg));
-                            float e0, e1;
-                            unf2(u, &e0, &e1);
-                            sum[0] = add2(sum[0], f2(ex2(e0), ex2(e1)));
-                            sum[1] = add2(sum[1], ex2_poly<5>(v));
+#pragma unroll
+                            for (int k = 0; k < 2; k++) {
+                                const ull z = fma2(f2(s[4 * j + 2 * k], s[4 * j + 2 * k + 1]), sl2,
+                                                   k ? f2(l4.z, l4.w) : f2(l4.x, l4.y));
+                                if ((2 * j + k) * kMassPoly % 8 < kMassPoly) {
+                                    sum[k] = add2(sum[k], ex2_poly(z));
+                                } else {
+                                    float e0, e1;
+                                    unf2(z, &e0, &e1);
+                                    sum[k] = add2(sum[k], f2(ex2(e0), ex2(e1)));
+                                }
+                            }
                         }
                     } else {
                         const int l0 = lo - c * 32, h0 = hi - c * 32;
@@ -954,7 +954,7 @@ mass_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                                 float e[4];
 #pragma unroll
                                 for (int k = 0; k < 4; k++)
-                                    e[k] = bits >> (4 * j + k) & 1 ? ex2(s[4 * j + k] * a.sl2 - lv[k]) : 0.f;
+                                    e[k] = bits >> (4 * j + k) & 1 ? ex2(s[4 * j + k] * a.sl2 + lv[k]) : 0.f;
                                 sum[0] = add2(sum[0], f2(e[0], e[1]));
                                 sum[1] = add2(sum[1], f2(e[2], e[3]));
                             }
@@ -969,7 +969,8 @@ mass_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             float s0, s1, s2, s3;
             unf2(sum[0], &s0, &s1);
             unf2(sum[1], &s2, &s3);
-            sh.key[x * 128 + r] = (s0 + s1) + (s2 + s3);
+            // two terms onto zero: the same whichever comes first
+            atomicAdd(&sh.key[x * 128 + r], (s0 + s1) + (s2 + s3));
             const bool whole = w.t0 == 0 && w.t1 == w.nt;
             const uint32_t bs = p.bs.d;
             // blocks of at most 128 keys belong to one group, larger ones to both
@@ -985,15 +986,18 @@ mass_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             meet();
             if (!ok) break;
             const uint32_t nb = both ? 1 : 128 / bs;
-            if (r < nb && !(both && x == 1)) {
-                float y = 0.f;
-                for (uint32_t k = 0; k < bs; k++) y += sh.key[x * 128 + r * bs + k];
+            if (y == 0 && r < nb && !(both && x == 1)) {
+                float v = 0.f;
+                for (uint32_t k = 0; k < bs; k++) {
+                    v += sh.key[x * 128 + r * bs + k];
+                    sh.key[x * 128 + r * bs + k] = 0.f;
+                }
                 const uint32_t lb = (both ? 0 : x * nb) + r;          // block of the unit
                 const uint32_t gb = w.key0() / bs + lb;
-                if (!whole) sp.ws[(size_t)(2 * blockIdx.x + (w.t0 == 0 ? 1 : 0)) * kMassSlot + lb] = y;
-                else if (gb < b.width) a.mass[((size_t)w.at.i * g.H + w.at.h) * b.width + gb] = y;
+                if (!whole) sp.ws[(size_t)(2 * blockIdx.x + (w.t0 == 0 ? 1 : 0)) * kMassSlot + lb] = v;
+                else if (gb < b.width) a.mass[((size_t)w.at.i * g.H + w.at.h) * b.width + gb] = v;
             }
-            if (w.t0 == 0) mass_zero_rest(w, b, p, a.mass, x * 128 + r, 256);
+            if (w.t0 == 0 && y == 0) mass_zero_rest(w, b, p, a.mass, x * 128 + r, 256);
             meet();
             live = w.next();
         }

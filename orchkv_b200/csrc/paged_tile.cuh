@@ -209,27 +209,22 @@ __device__ __forceinline__ ull mul2(ull a, ull b)
 // Two powers of two without the special function unit, for arguments below
 // 2^7: x = n + f with |f| <= 1/2 (adding 1.5 * 2^23 rounds x to n and leaves n
 // in the low bits), 2^f by a polynomial, n into the exponent.  Arguments below
-// -126 count as -126.  The polynomials minimise the largest relative error
-// over [-1/2, 1/2] (Remez exchange in double, coefficients rounded): 2.7e-6
-// (degree 4) and 2.1e-7 (degree 5) when evaluated in fp32, with means of
-// 4e-8 and 5e-8, so sums of many are off by about that.
-template <int DEG> __device__ __forceinline__ ull ex2_poly(ull x)
+// -126 count as -126.  The polynomial of degree 5 minimises the largest
+// relative error over [-1/2, 1/2] (Remez exchange in double, coefficients
+// rounded): 2.1e-7 when evaluated in fp32, 5e-8 on average, about what a sum
+// of many is off by.
+__device__ __forceinline__ ull ex2_poly(ull x)
 {
-    static_assert(DEG == 4 || DEG == 5, "");
     float a, b;
     unf2(x, &a, &b);
     x = f2(fmaxf(a, -126.f), fmaxf(b, -126.f));
     const ull t = add2(x, f2(12582912.f, 12582912.f));
     const ull f = fma2(add2(t, f2(-12582912.f, -12582912.f)), f2(-1.f, -1.f), x);
-    constexpr float c4[5] = {0x1.ffffe8p-1f, 0x1.62e0dcp-1f, 0x1.ec06dap-3f, 0x1.ca1444p-5f, 0x1.3997d6p-7f};
-    constexpr float c5[6] = {0x1.000002p+0f, 0x1.62e428p-1f, 0x1.ebf918p-3f, 0x1.c6b6e4p-5f, 0x1.3d0c52p-7f,
-                             0x1.5c08e6p-10f};
-    ull p = DEG == 4 ? f2(c4[4], c4[4]) : f2(c5[5], c5[5]);
+    constexpr float c[6] = {0x1.000002p+0f, 0x1.62e428p-1f, 0x1.ebf918p-3f, 0x1.c6b6e4p-5f, 0x1.3d0c52p-7f,
+                            0x1.5c08e6p-10f};
+    ull p = f2(c[5], c[5]);
 #pragma unroll
-    for (int k = DEG - 1; k >= 0; k--) {
-        const float c = DEG == 4 ? c4[k < 5 ? k : 0] : c5[k];
-        p = fma2(p, f, f2(c, c));
-    }
+    for (int k = 4; k >= 0; k--) p = fma2(p, f, f2(c[k], c[k]));
     float ta, tb;
     unf2(t, &ta, &tb);
     unf2(p, &a, &b);
