@@ -21,7 +21,7 @@
 #ifndef ORCHKV_PAGED_OPS_H
 #define ORCHKV_PAGED_OPS_H
 
-#include "kv_types.h"
+#include "orchkv_api.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -135,6 +135,21 @@ size_t orchkv_paged_block_mass_workspace(const orchkv_pages_t *pages, const orch
                                          const orchkv_mass_args_t *args);
 int orchkv_paged_block_mass(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
                             const orchkv_mass_args_t *args, void *workspace, size_t bytes, void *stream);
+
+/* The data plane's GPU pool as pages of one head each, for requests of
+ * n_kv_heads KV heads. */
+int orchkv_pool_pages(uint32_t n_kv_heads, orchkv_pages_t *out);
+
+/* The tables of these operators for one layer of the given requests (which
+ * all have n_kv_heads KV heads and the same n_layers), device memory: table [n][n_kv_heads]
+ * [ceil(row_len / tokens_per_block)] the GPU slab of each block, -1 where a
+ * block does not exist or lies on another tier; lens [n] (may be NULL) the
+ * tokens held.  New tokens get their blocks first: orchkv_append_token_batch
+ * (one token, every layer) and orchkv_prefill (one layer) with NULL data
+ * allocate and count them, orchkv_paged_append then writes them.
+ * Asynchronous on the data plane's stream. */
+int orchkv_slab_table(kv_request_ctx_t *const *ctxs, uint32_t n, uint32_t layer_id, uint32_t n_kv_heads,
+                      uint32_t row_len, int32_t *table, int32_t *lens);
 
 /* ORCHKV_ERR_CUDA once a wait inside one of these kernels has run out (2 s;
  * its call's results are then not complete), ORCHKV_OK otherwise.

@@ -154,6 +154,8 @@ _SIGS = {
     "orchkv_paged_attend_workspace": (C.c_size_t, [P(Pages), P(Batch), P(AttendArgs)]),
     "orchkv_paged_attend": (i32, [P(Pages), P(Batch), P(AttendArgs), vp, C.c_size_t, vp]),
     "orchkv_paged_status": (i32, []),
+    "orchkv_pool_pages": (i32, [u32, P(Pages)]),
+    "orchkv_slab_table": (i32, [P(vp), u32, u32, u32, u32, vp, vp]),
     "orchkv_paged_block_mass_workspace": (C.c_size_t, [P(Pages), P(Batch), P(MassArgs)]),
     "orchkv_paged_block_mass": (i32, [P(Pages), P(Batch), P(MassArgs), vp, C.c_size_t, vp]),
     # data plane

@@ -28,6 +28,7 @@
 
 #include "kernels.h"
 #include "orchkv/orchkv_api.h"
+#include "orchkv/paged_ops.h"
 #include "pool.h"
 #include "tm_internal.h"
 
@@ -1762,6 +1763,39 @@ int orchkv_block_id_table(kv_request_ctx_t *const *ctxs, uint32_t n, uint32_t ro
     int rc = upload_regions(ctxs, n, &L, &H, &mbph);
     if (rc) return rc;
     return launch_id_table(g.p, g.regions_dev, n, L, H, mbph, row_len, out, g.stream);
+}
+
+int orchkv_pool_pages(uint32_t n_kv_heads, orchkv_pages_t *out)
+{
+    std::lock_guard<std::recursive_mutex> lk(g.mu);
+    if (!g.inited) return ORCHKV_ERR_INIT;
+    if (!out || n_kv_heads == 0) return ORCHKV_ERR_INVALID;
+    const size_t e = dtype_size(g.cfg.dtype);
+    out->k = g.p.gpu_base;
+    out->v = g.p.gpu_base + g.p.half;
+    out->page_stride = (int64_t)(g.p.slab / e);
+    out->head_stride = 0;
+    out->token_stride = (int64_t)g.cfg.d_head;
+    out->n_pages = g.p.g_total;
+    out->page_tokens = g.p.tpb;
+    out->n_kv_heads = n_kv_heads;
+    out->d_head = g.cfg.d_head;
+    out->dtype = (int)g.cfg.dtype;
+    return ORCHKV_OK;
+}
+
+int orchkv_slab_table(kv_request_ctx_t *const *ctxs, uint32_t n, uint32_t layer_id, uint32_t n_kv_heads,
+                      uint32_t row_len, int32_t *table, int32_t *lens)
+{
+    OKV_RANGE("orchkv_slab_table");
+    std::lock_guard<std::recursive_mutex> lk(g.mu);
+    if (!g.inited) return ORCHKV_ERR_INIT;
+    if (!table || row_len == 0) return ORCHKV_ERR_INVALID;
+    uint32_t L, H, mbph;
+    int rc = upload_regions(ctxs, n, &L, &H, &mbph);
+    if (rc) return rc;
+    if (layer_id >= L || n_kv_heads != H) return ORCHKV_ERR_INVALID;
+    return launch_slab_table(g.p, g.regions_dev, n, L, H, mbph, layer_id, row_len, table, lens, g.stream);
 }
 
 int orchkv_block_info(kv_request_ctx_t *ctx, uint32_t l, uint32_t h, uint32_t bi,

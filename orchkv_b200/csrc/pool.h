@@ -181,6 +181,11 @@ int launch_conflicts(const PoolDev &p, const MigPlan &promote, const SortScratch
 int launch_id_table(const PoolDev &p, uint32_t *const *regions, uint32_t n, uint32_t L,
                     uint32_t H, uint32_t mbph, uint32_t row_len, uint32_t *out,
                     cudaStream_t s);
+// Slabs and token counts of one layer: table [n][H][ceil(row_len/tpb)], lens [n]
+// (may be null).
+int launch_slab_table(const PoolDev &p, uint32_t *const *regions, uint32_t n, uint32_t L, uint32_t H,
+                      uint32_t mbph, uint32_t l, uint32_t row_len, int32_t *table, int32_t *lens,
+                      cudaStream_t s);
 // Batched storage moves: triples lhb[3n] -> out[3n] = {id, loc word, flags}.
 int launch_lhb_lookup(const PoolDev &p, const ReqDev &r, const uint32_t *lhb, uint32_t n,
                       uint32_t *out, cudaStream_t s);

@@ -917,6 +917,30 @@ __global__ void id_table_kernel(PoolDev p, uint32_t *const *regions, uint32_t n,
     }
 }
 
+// GPU slab of every block of one layer (-1 where a block does not exist or lies
+// on another tier), and the tokens held: the tables of the paged operators.
+__global__ void slab_table_kernel(PoolDev p, uint32_t *const *regions, uint32_t n, uint32_t L, uint32_t H,
+                                  uint32_t mbph, uint32_t l, uint32_t nb, int32_t *table, int32_t *lens)
+{
+    const unsigned long long total = (unsigned long long)n * H * nb;
+    const unsigned long long t0 = (unsigned long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (lens)
+        for (unsigned long long i = t0; i < n; i += (unsigned long long)gridDim.x * blockDim.x)
+            lens[i] = (int32_t)regions[i][1 + l];
+    for (unsigned long long e = t0; e < total; e += (unsigned long long)gridDim.x * blockDim.x) {
+        const uint32_t b = (uint32_t)(e % nb), i = (uint32_t)(e / nb / H), hh = (uint32_t)(e / nb % H);
+        const uint32_t *reg = regions[i];
+        int32_t slab = -1;
+        if (b < (reg[1 + l] + p.tpb - 1) / p.tpb && b < mbph) {
+            const uint32_t id = reg[1 + L + ((size_t)l * H + hh) * mbph + b];
+            if (id < p.max_blocks && loc_tier(p.loc[id]) == TIER_GPU_HBM &&
+                OKV_IN(p.chk, loc_slab(p.loc[id]), p.g_total))
+                slab = (int32_t)loc_slab(p.loc[id]);
+        }
+        table[e] = slab;
+    }
+}
+
 // ---------------------------------------------------------------------------
 // Request teardown (src/api/orchkv_api.cu:149-183): free slabs and ids in
 // (layer, head, block) order.  One CTA, contiguous chunks per thread.
@@ -1364,6 +1388,17 @@ int launch_id_table(const PoolDev &p, uint32_t *const *regions, uint32_t n, uint
     if (g > 148 * 16) g = 148 * 16;
     if (g == 0) g = 1;
     id_table_kernel<<<g, 256, 0, s>>>(p, regions, n, L, H, mbph, nb, out); note_launches(1);
+    OKV_CUDA_TRY(cudaGetLastError());
+    return ORCHKV_OK;
+}
+
+int launch_slab_table(const PoolDev &p, uint32_t *const *regions, uint32_t n, uint32_t L, uint32_t H,
+                      uint32_t mbph, uint32_t l, uint32_t row_len, int32_t *table, int32_t *lens,
+                      cudaStream_t s)
+{
+    const uint32_t nb = (row_len + p.tpb - 1) / p.tpb;
+    slab_table_kernel<<<copy_grid((unsigned long long)n * H * nb, 256), 256, 0, s>>>(p, regions, n, L, H, mbph, l, nb, table,
+                                                                                     lens); note_launches(1);
     OKV_CUDA_TRY(cudaGetLastError());
     return ORCHKV_OK;
 }

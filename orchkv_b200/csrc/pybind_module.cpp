@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "orchkv/orchkv_api.h"
+#include "orchkv/paged_ops.h"
 #include "orchkv/tiered_manager.h"
 
 namespace py = pybind11;
@@ -316,6 +317,15 @@ PYBIND11_MODULE(orchkv_core, m)
               return orchkv_block_id_table(l.data(), (uint32_t)l.size(), row_len, P<uint32_t>(out));
           },
           py::arg("ctxs"), py::arg("row_len"), py::arg("out_ptr"));
+    m.def("slab_table",
+          [](const std::vector<uintptr_t> &ctxs, uint32_t layer, uint32_t heads, uint32_t row_len,
+             uintptr_t table, uintptr_t lens) {
+              auto l = ctx_list(ctxs);
+              return orchkv_slab_table(l.data(), (uint32_t)l.size(), layer, heads, row_len, P<int32_t>(table),
+                                       P<int32_t>(lens));
+          },
+          py::arg("ctxs"), py::arg("layer_id"), py::arg("n_kv_heads"), py::arg("row_len"), py::arg("table_ptr"),
+          py::arg("lens_ptr") = 0);
     m.def("evict_batch_to_dram",
           [](uintptr_t ids, uintptr_t count, uint32_t max_n, uintptr_t result) {
               return orchkv_evict_batch_to_dram(P<const uint32_t>(ids), P<const uint32_t>(count),

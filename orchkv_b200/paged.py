@@ -26,11 +26,13 @@ state between calls.  The operators have no gradient.
 """
 from __future__ import annotations
 
+import ctypes as C
 import math
 
 import torch
 
-from . import torch_ops
+from . import core, lib, torch_ops
+from ._lib import Pages
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
@@ -173,6 +175,27 @@ class PagedKV:
         self._ops = torch_ops().Pages(device, k_ptr, v_ptr, *strides, n_pages, tokens, heads or 0,
                                       head_dim, _DTYPES[dtype])
 
+    @classmethod
+    def over_pool(cls) -> "PagedKV":
+        """The pages of the data plane's GPU pool (orchkv_init): slabs of one
+        head, with tables from ``pool_table``.  Valid until its shutdown."""
+        pg = Pages()
+        rc = lib().orchkv_pool_pages(1, C.byref(pg))
+        if rc != 0:
+            raise RuntimeError(f"orchkv_pool_pages failed: {rc}")
+        dtype = {v: k for k, v in _DTYPES.items()}.get(pg.dtype)
+        _need(dtype is not None, "the pool's type is not supported")
+        _need(pg.d_head <= 256 and pg.d_head * dtype.itemsize % 16 == 0,
+              "d_head must be at most 256 and a multiple of 16 bytes")
+        self = cls.__new__(cls)
+        self.k = self.v = None
+        self.layout = "slab"
+        device = C.cast(lib().orchkv_gpu_tier(), C.POINTER(C.c_int))[0]   # its first field
+        self._set(device, pg.k, pg.v,
+                  (pg.page_stride, pg.head_stride, pg.token_stride), pg.n_pages, pg.page_tokens, None,
+                  pg.d_head, dtype)
+        return self
+
     def append(self, k, v, table, lens, starts, *, q=None, rotary: Rotary | None = None,
                positions=None, q_norm=None, k_norm=None, eps: float = 1e-6, q_out=None):
         """The new tokens' k, v [rows, KV heads, head_dim] into the pages; lens
@@ -205,3 +228,24 @@ class PagedKV:
         heads and the block's tokens of exp(scale * q k - lse), with the lse
         that attend returned for the same arguments."""
         return self._ops.block_mass(q, lse, table, lens, starts, scale, window, max_new, out)
+
+
+def pool_table(requests, layer: int, row_len: int, n_kv_heads: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Table [requests, KV heads, blocks] and lens of one layer of data-plane
+    requests (handles of ``orchkv_core.request_create``): the slabs of the
+    blocks that lie on the GPU, -1 for the others, for the first `row_len`
+    tokens.  Runs on the data plane's stream, which is the current stream
+    after ``orchkv_core.set_stream`` and ordered with the default stream
+    otherwise; take it again after blocks were allocated or moved."""
+    cpp, pg = core(), Pages()
+    rc = lib().orchkv_pool_pages(max(n_kv_heads, 1), C.byref(pg))
+    if rc != 0:
+        raise RuntimeError(f"orchkv_pool_pages failed: {rc}")
+    _need(n_kv_heads > 0 and row_len > 0 and len(requests) > 0, "requests, heads and row_len must not be 0")
+    table = torch.empty(len(requests), n_kv_heads, -(-row_len // pg.page_tokens), dtype=torch.int32,
+                        device="cuda")
+    lens = torch.empty(len(requests), dtype=torch.int32, device="cuda")
+    rc = cpp.slab_table(list(requests), layer, n_kv_heads, row_len, table.data_ptr(), lens.data_ptr())
+    if rc != 0:
+        raise RuntimeError(f"orchkv_slab_table failed: {rc}")
+    return table, lens

@@ -422,3 +422,95 @@ def test_offsets_past_32_bits(cuda):
     c["k"][:, :, :] = 1.5
     kv(c).append(c["k"], c["v"], c["table"], c["lens"], c["starts"])
     assert (kp[int(c["table"][0, 200 // block]), 200 % block] == 1.5).all()
+
+
+# ---- refusals --------------------------------------------------------------------
+
+def test_refusals(cuda):
+    """Arguments that do not fit raise before anything is launched."""
+    torch = cuda
+    from orchkv_b200 import paged
+    c = P.make(torch, [2, 1], [5, 30], hq=4, hk=2)
+    x = kv(c)
+    a = (c["table"], c["lens"], c["starts"])
+    cpu, bad = c["q"].cpu(), torch.zeros(3, 5, 128, dtype=c["dt"], device="cuda")
+    lse = torch.zeros(3, 4, device="cuda")
+    calls = [
+        (lambda: x.attend(c["q"].float(), *a), "dtype"),
+        (lambda: x.attend(c["q"][:, :, :64], *a), "must be"),
+        (lambda: x.attend(c["q"][0], *a), "must be"),
+        (lambda: x.attend(bad, *a), "share"),
+        (lambda: x.attend(cpu, *a), "device"),
+        (lambda: x.attend(c["q"].transpose(1, 2).contiguous().transpose(1, 2), *a), "contiguous"),
+        (lambda: x.attend(torch.zeros(3, 4, 132, dtype=c["dt"], device="cuda")[:, :, :128], *a), "16 bytes"),
+        (lambda: x.attend(c["q"], c["table"].long(), *a[1:]), "int32"),
+        (lambda: x.attend(c["q"], c["table"][0], *a[1:]), "table must be"),
+        (lambda: x.attend(c["q"], c["table"][:, :0], *a[1:]), "no blocks"),
+        (lambda: x.attend(c["q"], c["table"].t().contiguous().t(), *a[1:]), "contiguous"),
+        (lambda: x.attend(c["q"], c["table"].cpu(), *a[1:]), "device"),
+        (lambda: x.attend(c["q"], c["table"], c["lens"][:1], c["starts"]), "entries"),
+        (lambda: x.attend(c["q"], c["table"], c["lens"], c["lens"]), "entries"),
+        (lambda: x.attend(c["q"], *a, window=-1), "window"),
+        (lambda: x.attend(c["q"], *a, max_new=-1), "max_new"),
+        (lambda: x.attend(c["q"], *a, out=c["q"][:2]), "out must be"),
+        (lambda: x.attend(c["q"].float().requires_grad_().to(c["dt"]), *a), "gradient"),
+        (lambda: x.append(c["k"][:2], c["v"], *a), "v must be"),
+        (lambda: x.append(c["q"], c["v"], *a), "k must be"),
+        (lambda: x.append(c["k"], c["v"], *a, q_norm=c["k"][0, 0]), "go with q"),
+        (lambda: x.append(c["k"], c["v"], *a, k_norm=c["k"][0]), "k_norm"),
+        (lambda: x.append(c["k"], c["v"], *a, k_norm=c["k"][0, 0].float()), "k_norm"),
+        (lambda: x.append(c["k"], c["v"], *a, positions=torch.zeros(2, device="cuda", dtype=torch.int32)),
+         "positions"),
+        (lambda: x.append(c["k"], c["v"], *a, positions=torch.zeros(3, device="cuda")), "positions"),
+        (lambda: x.append(c["k"], c["v"], *a, rotary=paged.Rotary(256)), "wider"),
+        (lambda: x.append(c["k"], c["v"], *a, rotary=paged.Rotary(128, device="cpu")), "wider|device"),
+        (lambda: x.block_mass(c["q"], lse[:, :2], *a), "lse"),
+        (lambda: x.block_mass(c["q"], lse.double(), *a), "lse"),
+        (lambda: x.block_mass(c["q"], lse, *a, out=lse), "out must be"),
+    ]
+    for fn, msg in calls:
+        with pytest.raises(ValueError, match=msg):
+            fn()
+    with pytest.raises(TypeError):
+        x.attend(None, *a)
+    from orchkv_b200 import lib
+    assert lib().orchkv_paged_status() == 0
+
+
+def test_nothing_to_do(cuda):
+    torch = cuda
+    c = P.make(torch, [0, 0], [5, 30], hq=4, hk=2)
+    out, lse = attend(c)
+    assert out.shape == (0, 4, 128) and lse.shape == (0, 4)
+    assert kv(c).append(c["k"], c["v"], c["table"], c["lens"], c["starts"]) is None
+    mass = kv(c).block_mass(c["q"], lse, c["table"], c["lens"], c["starts"])
+    assert (mass == 0).all()
+    none = [t[:0].contiguous() for t in (c["table"], c["lens"])] + [c["starts"][:1].contiguous()]
+    assert kv(c).attend(c["q"], *none).shape == (0, 4, 128)
+    assert kv(c).block_mass(c["q"], lse, *none).shape == (0, 2, c["table"].shape[1])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+@pytest.mark.parametrize("new", [1, 90])
+def test_scales_that_turn_or_drop_the_order(cuda, scale, new):
+    torch = cuda
+    c = P.make(torch, [new, 3], [200, 10], hq=8, hk=2, seed=new)
+    out, lse = attend(c, scale=scale)
+    P.check_attend(c, out, lse, scale)
+    mass = kv(c).block_mass(c["q"], lse, c["table"], c["lens"], c["starts"], scale=scale)
+    P.check_mass(c, mass, lse, scale)
+
+
+@pytest.mark.parametrize("hq,hk,block", [(28, 4, 16), (14, 2, 256), (12, 1, 8), (40, 1, 64), (3, 3, 32)])
+@pytest.mark.parametrize("window", [0, 200])
+def test_chunks_over_many_units(cuda, hq, hk, block, window):
+    """Chunks long enough that units are cut and joined, groups that do not
+    divide a tile, one head a KV head; masses of the same calls."""
+    torch = cuda
+    c = P.make(torch, [700, 1, 90], [900, 3000, 0], hq=hq, hk=hk, d=64, block=block, seed=hq)
+    out, lse = attend(c, window=window)
+    P.check_attend(c, out, lse, 64 ** -0.5, window)
+    mass = kv(c).block_mass(c["q"], lse, c["table"], c["lens"], c["starts"], window=window)
+    P.check_mass(c, mass, lse, 64 ** -0.5, window)
+    again = kv(c).block_mass(c["q"], lse, c["table"], c["lens"], c["starts"], window=window)
+    assert torch.equal(mass, again)
