@@ -106,8 +106,9 @@ typedef struct orchkv_attend_args {
  * of r's sequence up to r's own place that lie in a page (and in the
  * window), KV head h / (n_q_heads / n_kv_heads); lse[r, h] = the logarithm of
  * the softmax's denominator.  A row with no such token gets 0 and -infinity.
- * Keys and values of places no row attends to are not looked at; of the
- * places that only some rows of a call attend to, the values must be finite.
+ * What lies in places that a row does not attend to does not reach it, be it
+ * infinite or NaN; an infinite or NaN value reaches every row that does, as
+ * such or as NaN.
  * workspace: orchkv_paged_attend_workspace() bytes of device memory, 256-byte
  * aligned, of this call alone until it has run.  Asynchronous. */
 size_t orchkv_paged_attend_workspace(const orchkv_pages_t *pages, const orchkv_batch_t *batch,

@@ -2,6 +2,8 @@
 // the kernels with few query rows (paged_rows.cu).
 #pragma once
 
+#include <type_traits>
+
 #include "paged_split.cuh"
 
 namespace okv {
@@ -66,6 +68,31 @@ __device__ __forceinline__ float ex2(float x)
 }
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
+
+// Whether 16-bit values are all finite, a pair at a time: x * 0 is 0 for a finite
+// x and NaN for the others, and stays NaN in a sum.
+template <class T> struct Finite;
+template <> struct Finite<__nv_bfloat16> {
+    __nv_bfloat162 a = __floats2bfloat162_rn(0.f, 0.f);
+    __device__ __forceinline__ void see(uint32_t w)
+    {
+        a = __hfma2(*reinterpret_cast<__nv_bfloat162 *>(&w), __floats2bfloat162_rn(0.f, 0.f), a);
+    }
+    __device__ __forceinline__ bool none() const { return __low2float(a) == 0.f && __high2float(a) == 0.f; }
+};
+template <> struct Finite<__half> {
+    __half2 a = __floats2half2_rn(0.f, 0.f);
+    __device__ __forceinline__ void see(uint32_t w)
+    {
+        a = __hfma2(*reinterpret_cast<__half2 *>(&w), __floats2half2_rn(0.f, 0.f), a);
+    }
+    __device__ __forceinline__ bool none() const { return __low2float(a) == 0.f && __high2float(a) == 0.f; }
+};
+template <class T> __device__ __forceinline__ bool infinite(uint32_t w, int half)
+{
+    const uint32_t m = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+    return ((half ? w >> 16 : w) & m) == m;
+}
 
 // Offset of 16-byte column c of row r in a tile of rows of DP elements: the
 // column is exchanged within its row so that 8 rows of one column fall on

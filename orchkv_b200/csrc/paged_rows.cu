@@ -58,6 +58,51 @@ __device__ __forceinline__ void cluster_meet()
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Before a product with 16 keys that only some rows attend to: a weight of 0
+// times an infinite or NaN value would reach the rows that do not, so such
+// values become 0 and the results of the rows that do attend NaN.
+template <class T, int DP>
+__device__ __forceinline__ void drop_infinite(uint32_t vt, const RowInfo &r0, const RowInfo &r1, int k0,
+                                              uint32_t have, float (*acc)[4])
+{
+    const uint32_t lane = threadIdx.x & 31;
+    Finite<T> fin;
+#pragma unroll
+    for (int k = 0; k < DP / 16; k++) {
+        uint32_t w[4];
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(vt + (k * 32 + lane) * 16));
+#pragma unroll
+        for (int j = 0; j < 4; j++) fin.see(w[j]);
+    }
+    if (__all_sync(0xFFFFFFFFu, fin.none())) return;
+#pragma unroll
+    for (int n = 0; n < DP / 8; n++)
+#pragma unroll 1
+        for (uint32_t c = 0; c < 16; c++) {
+            const int key = k0 + (int)c;
+            uint32_t w;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(vt + swz<DP>(c, n) + (lane & 3) * 4));
+            if (!(have >> c & 1)) continue;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                if (infinite<T>(w, j)) {
+                    if (key <= r0.hi && key >= r0.lo) acc[n][j] = NAN;
+                    if (key <= r1.hi && key >= r1.lo) acc[n][2 + j] = NAN;
+                }
+        }
+    __syncwarp();
+#pragma unroll 1
+    for (uint32_t e = lane; e < 16 * DP / 2; e += 32) {
+        uint32_t w;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(vt + e * 4));
+        if (infinite<T>(w, 0)) w &= 0xFFFF0000u;
+        if (infinite<T>(w, 1)) w &= 0xFFFFu;
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(vt + e * 4), "r"(w) : "memory");
+    }
+    __syncwarp();
+}
+
 // CL: a unit is one cluster of `split` CTAs, which share its keys equally and
 // join their parts over each other's shared memory; else the CTAs share the
 // whole call's work and join_kernel adds cut units.
@@ -217,6 +262,7 @@ attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint
                             acc[n][3] *= f[1];
                         }
                     }
+                    if (k0 < all_lo || k0 + 15 > all_hi) drop_infinite<T, DP>(vt, r0, r1, k0, have, acc);
                     // matrices: keys lo | hi | lo | hi, columns 0-7 | 0-7 | 8-15 | 8-15
                     const uint32_t r = lane & 15, cx = lane >> 4;
 #pragma unroll

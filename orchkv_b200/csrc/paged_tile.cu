@@ -48,6 +48,7 @@ struct TileShared {
     ull full[8], empty[8], s_full[2], p_full[2], q_full[2], o_full[2], s_free, fix, drain;
     uint32_t tmem;
     int dead;
+    int odd[kMeta];                        // of a unit: values that are not finite behind some row's mask
     alignas(16) uint32_t mask[kMeta][4];   // columns of a tile that hold a token
     SplitShared split;
 };
@@ -106,7 +107,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         const uint32_t bs = p.bs.d, per = bs < kK ? kK / bs : 1, box = bs < kK ? bs : kK;
         const uint32_t page_bytes = box * 128, all_pages = per == 32 ? 0xFFFFFFFFu : (1u << per) - 1;
         constexpr uint32_t halves = DP / 64;
-        uint32_t st = is_v ? 1 : 0, ph = 0, fix_ph = 0, tile_no = 0;
+        uint32_t st = is_v ? 1 : 0, ph = 0, fix_ph = 0, tile_no = 0, u_no = 0;
         const bool one = elect_one();
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -116,6 +117,10 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         do {
             const uint32_t h = w.at.h, i = w.at.i;
             const int zh = by_head ? 0 : (int)h;
+            // keys that every row of the unit attends to
+            const int all_hi = row_info(g, w.s, h, w.at.rt * kR).hi;
+            const int all_lo = row_info(g, w.s, h, w.at.rt * kR + w.live() - 1).lo;
+            if (is_v && lane == 0) sh.odd[u_no % kMeta] = 0;
             auto page = [&](uint32_t t) {                  // lane q: page q of tile t
                 if (t >= w.t1 || lane >= per) return -1;
                 const uint32_t k0 = (w.first + t) * kK + lane * bs;
@@ -144,7 +149,8 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                     else if (lim < 32) word &= (1u << lim) - 1;
                 }
                 const uint32_t full = smem_addr(&sh.full[st]), dst = ring + st * Cfg::tile;
-                const bool fix = is_v && part;
+                const bool some = (int)k0 < all_lo || (int)(k0 + kK) - 1 > all_hi;
+                const bool fix = is_v && (part || some);
                 const uint32_t bar = fix ? smem_addr(&sh.fix) : full;
                 wait(smem_addr(&sh.empty[st]), ph ^ 1);
                 if (!ok) break;
@@ -178,6 +184,32 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                                     asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
                                                      dst + x * kK * 128 + r * 128 + c * 16), "r"(0) : "memory");
                     }
+                    __syncwarp();
+                    // nor would 0 times an infinite value of a token that only
+                    // some rows attend to: it becomes 0 here, and the results of
+                    // the rows that do attend to it NaN at the unit's end
+                    if (ok && some) {
+                        Finite<T> fin;
+#pragma unroll 8
+                        for (uint32_t e = lane; e < Cfg::tile / 16; e += 32) {
+                            uint32_t v[4];
+                            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(dst + e * 16));
+#pragma unroll
+                            for (int j = 0; j < 4; j++) fin.see(v[j]);
+                        }
+                        if (!__all_sync(0xFFFFFFFFu, fin.none())) {
+#pragma unroll 1
+                            for (uint32_t e = lane; e < Cfg::tile / 4; e += 32) {
+                                uint32_t v;
+                                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(dst + e * 4));
+                                if (infinite<T>(v, 0)) v &= 0xFFFF0000u;
+                                if (infinite<T>(v, 1)) v &= 0xFFFFu;
+                                asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + e * 4), "r"(v) : "memory");
+                            }
+                            if (lane == 0) sh.odd[u_no % kMeta] = 1;
+                        }
+                    }
                     fence_async();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(full);
@@ -186,6 +218,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 if (st >= ST) { st -= ST; ph ^= 1; }
                 pg = nxt;
             }
+            u_no++;
         } while (ok && w.next());
         if (!ok) {
             // leave no copy in flight behind
@@ -292,7 +325,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         const uint32_t r = threadIdx.x - 128 - x * 128;    // row of the half
         const uint32_t lanes = (wid & 3) << 21;            // first lane of this warp, in a TMEM address
         const uint32_t S = tm + kS + lanes, P = tm + (x ? kP1 : kP0) + lanes, O = tm + 256 + x * 128 + lanes;
-        uint32_t s_ph = 0, o_ph = 0, tile_no = 0;
+        uint32_t s_ph = 0, o_ph = 0, tile_no = 0, u_no = 0;
         const ull sl2 = f2(a.sl2, a.sl2);
 
         auto load_q = [&](const Walk &u) {
@@ -314,6 +347,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         bool live = true;
         while (live && x == 1 && w.live() <= 128) {
             tile_no += w.t1 - w.t0;
+            u_no++;
             live = w.next();
         }
         if (live) load_q(w);
@@ -423,9 +457,10 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             // the next unit's queries while the last products run, then the rows
             Walk u = w;
             live = u.next();
-            uint32_t skipped = 0;
+            uint32_t skipped = 0, units = 1;
             while (live && x == 1 && u.live() <= 128) {
                 skipped += u.t1 - u.t0;
+                units++;
                 live = u.next();
             }
             if (live) load_q(u);
@@ -438,7 +473,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             unf2(l2[0], &la, &lb);
             unf2(l2[1], &lc, &ld);
             const float L = (la + lb) + (lc + ld);
-            const bool whole = w.t0 == 0 && w.t1 == w.nt;
+            const bool whole = w.t0 == 0 && w.t1 == w.nt, odd = sh.odd[u_no % kMeta] != 0;
             const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
             float *sl = slot_of(sp.ws, 2 * blockIdx.x + (w.t0 == 0 ? 1 : 0), kR, p.D);
             char *dst = a.out.p + (long long)ri.row * a.out.row_b + (long long)ri.head * a.out.head_b;
@@ -447,6 +482,26 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 float o[32];
                 tm_ld32(O + c * 32, o);
                 tm_wait_ld();
+                if (odd && ri.row >= 0) {
+                    // rare: look the tokens over that only some rows attend to
+                    const int u_hi = row_info(g, w.s, w.at.h, w.at.rt * kR).hi;
+                    const int u_lo = row_info(g, w.s, w.at.h, w.at.rt * kR + w.live() - 1).lo;
+                    const int key_a = max((int)((w.first + w.t0) * kK), ri.lo);
+                    const int key_e = min((int)((w.first + w.t1) * kK) - 1, ri.hi);
+                    for (int key = key_a; key <= key_e; key++) {
+                        const int tile0 = key / (int)kK * (int)kK;
+                        if (tile0 >= u_lo && tile0 + (int)kK - 1 <= u_hi) continue;
+                        const uint32_t blk = (uint32_t)key / p.bs;
+                        const int pg = page_of(b, p.n_pages, w.at.i, w.at.h, blk);
+                        if (pg < 0) continue;
+                        const T *v = (const T *)(p.v + pg * p.page_b + w.at.h * p.head_b +
+                                                 (long long)((uint32_t)key - blk * p.bs.d) * p.tok_b) + c * 32;
+#pragma unroll
+                        for (int j = 0; j < 32; j++)
+                            if ((uint32_t)(c * 32 + j) < p.D && !isfinite(to_f(v[j]))) o[j] = NAN;
+                    }
+                }
+                __syncwarp();
                 if (ri.row >= 0 && whole) {
 #pragma unroll
                     for (int j = 0; j < 32; j++) o[j] *= inv;
@@ -475,6 +530,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             }
             tm_before();
             tile_no += skipped;
+            u_no += units;
             w.at = u.at;
             w.s = u.s;
             w.RT = u.RT;

@@ -197,6 +197,36 @@ def test_attend_infinite_and_nan_keys_behind_the_mask(cuda, new, dtype):
         P.check_attend(c, out, lse, 128 ** -0.5)
 
 
+@pytest.mark.parametrize("new,held", [(1, 200), (3, 130), (5, 27), (9, 700), (200, 130), (700, 300)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("window", [0, 40])
+def test_attend_infinite_values_reach_their_rows_alone(cuda, new, held, dtype, bad, window):
+    """A value that is infinite or NaN at one token (and one far before every
+    window): the rows that attend to it, and they alone, are not finite there;
+    every other number is as without it."""
+    torch = cuda
+    c = P.make(torch, [new, 2], [held, 60], hq=14, hk=2, dtype=dtype, seed=new)
+    want, wl = attend(c, window=window)
+    at = held + new // 2                          # the value's token
+    page = c["table"][0].tolist()
+    c["vp"][page[at // 16], at % 16, :, 7:10] = bad
+    if window:
+        c["vp"][page[0], 0] = bad                 # token 0: outside all windows but the first rows'
+    out, lse = attend(c, window=window)
+    assert torch.equal(lse, wl)
+    for r in range(new + 2):
+        sees = r < new and held + r >= at and (not window or held + r < at + window)
+        first = bool(window) and r < new and held + r < window
+        cols = torch.zeros(128, dtype=torch.bool, device="cuda")
+        if sees:
+            cols[7:10] = True
+        if first:
+            cols[:] = True
+        assert (~torch.isfinite(out[r][:, cols])).all(), r
+        assert torch.equal(out[r][:, ~cols], want[r][:, ~cols]), r
+
+
 def test_attend_large_scores(cuda):
     """Scores in the hundreds: the maximum moves all the time."""
     torch = cuda
