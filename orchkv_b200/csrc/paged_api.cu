@@ -78,14 +78,32 @@ RowsDev rows_dev(const orchkv_rows_t &r, size_t e)
     return RowsDev{(char *)r.p, r.row_stride * (long long)e, r.head_stride * (long long)e};
 }
 
-// Sequences with more packed rows than this go to the tile kernel, in calls
-// that may have any.
-constexpr uint32_t kFewRows = 64;
+// Which sequences go to the attention's tile kernel: none in calls whose row
+// tiles (16 packed rows) times key tiles (64 keys) are at most kSmall for each
+// of the few-row kernel's 296 places, where the second pair of launches costs
+// more than the tensor cores gain; else those with more than kFewRows packed
+// rows.  One request of 48 tokens over 500, 32/8 heads: 13.8 us against 26.1 by
+// the tile kernel; 8 requests of 12 over 500, 28/4 heads: 15.4 against 33.4; one
+// of 48 over 4000 (19 a place): 44.3 against 59.3; 8 of 12 over 4000 (41): 68.3
+// against 46.8.
+constexpr uint32_t kFewRows = 32;
+constexpr uint64_t kSmall = 24;
+// The masses' tile kernel has one product to do and two small launches: it takes
+// every sequence of more rows than this.  48 rows over 500: 8.7 us against 13.5
+// by the tile kernel; 96 rows: 15.2 against 14.3; 400 rows: 56.7 against 15.4.
+constexpr uint32_t kFewMassRows = 64;
+
+bool small_call(const orchkv_pages_t *p, const orchkv_batch_t *b, uint64_t G, uint64_t keys)
+{
+    const uint64_t units = p->n_kv_heads * (b->n_rows * G / 16 + b->n_seqs);
+    return units * ((keys + 63) / 64) <= kSmall * 296;
+}
 
 // What one attend call launches, from what the host knows of it.
 struct AttendPlan {
     SplitDev rows, tile;     // ctas 0: not launched
     ClassDev few, many;
+    bool no_rows;
     size_t bytes;
 };
 
@@ -95,13 +113,17 @@ AttendPlan plan_attend(const orchkv_pages_t *p, const orchkv_batch_t *b, const o
     const uint64_t G = args->n_q_heads / p->n_kv_heads, H = p->n_kv_heads;
     const uint64_t keys = (uint64_t)b->table_width * p->page_tokens;
     const uint64_t most = (uint64_t)(b->max_new < b->n_rows ? b->max_new : b->n_rows) * G;
-    const bool tile = most > kFewRows && attend_tile_takes(pages_dev(p), p->dtype, args->scale);
+    const bool tile = most > kFewRows && !small_call(p, b, G, keys) &&
+                      attend_tile_takes(pages_dev(p), p->dtype, args->scale);
     const uint32_t R = p->dtype == DTYPE_FP32 ? kSimtRows : kRowsRows;
     uint64_t units = H * (b->n_rows * G / R + b->n_seqs);
     if (tile) units = std::min(units, H * b->n_seqs * (kFewRows / R));
     pl.few = ClassDev{0, tile ? kFewRows : 0xFFFFFFFFu};
     pl.many = ClassDev{kFewRows, 0xFFFFFFFFu};
-    if (p->dtype == DTYPE_FP32)
+    pl.no_rows = tile && b->n_seqs == 1;     // one sequence is of one kind: one pair of launches
+    if (pl.no_rows)
+        pl.many.min_rows = 0;
+    else if (p->dtype == DTYPE_FP32)
         pl.rows.ctas = attend_simt_ctas(units, keys);
     else
         pl.rows = attend_rows_split(p->d_head, b->n_seqs, p->n_kv_heads,
@@ -128,10 +150,10 @@ MassPlan plan_mass(const orchkv_pages_t *p, const orchkv_batch_t *b, const orchk
     const uint32_t G = args->n_q_heads / p->n_kv_heads;
     const uint64_t keys = (uint64_t)b->table_width * p->page_tokens;
     const uint64_t new_rows = b->max_new < b->n_rows ? b->max_new : b->n_rows;
-    const bool tile = new_rows * G > kFewRows &&
+    const bool tile = new_rows * G > kFewMassRows &&
                       mass_tile_takes(pages_dev(p), p->dtype, args->scale, rows_dev(args->q, e), G);
-    pl.few = ClassDev{0, tile ? kFewRows : 0xFFFFFFFFu};
-    pl.many = ClassDev{kFewRows, 0xFFFFFFFFu};
+    pl.few = ClassDev{0, tile ? kFewMassRows : 0xFFFFFFFFu};
+    pl.many = ClassDev{kFewMassRows, 0xFFFFFFFFu};
     if (tile)
         pl.tile.ctas = mass_tile_ctas((uint64_t)p->n_kv_heads * b->n_seqs * ((keys + 255) / 256), new_rows * G);
     pl.bytes = ((size_t)2 * pl.tile.ctas * kMassSlot * sizeof(float) + 255) & ~size_t(255);
@@ -207,7 +229,8 @@ int orchkv_paged_attend(const orchkv_pages_t *pages, const orchkv_batch_t *batch
     pl.rows.ws = pl.tile.ws = (float *)workspace;
     const cudaStream_t st = (cudaStream_t)stream;
     if (pages->dtype == DTYPE_FP32) return launch_attend_simt(p, b, a, pl.few, pl.rows, st);
-    const int rc = launch_attend_rows(pages->dtype, p, b, a, pl.few, pl.rows, st);
+    int rc = ORCHKV_OK;
+    if (!pl.no_rows) rc = launch_attend_rows(pages->dtype, p, b, a, pl.few, pl.rows, st);
     if (rc || pl.tile.ctas == 0) return rc;
     return launch_attend_tile(pages->dtype, p, b, a, pl.many, pl.tile, st);
 }

