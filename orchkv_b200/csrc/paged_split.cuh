@@ -271,14 +271,14 @@ __device__ __forceinline__ float *slot_of(float *ws, uint32_t slot, uint32_t R, 
 }
 __host__ __device__ inline size_t slot_floats(uint32_t R, uint32_t D) { return (size_t)R * (D + 2); }
 
-// The slots of the pieces of the unit that boundary c (at position `at`, offset
-// `off` of its sequence) is the first to cut, in key order: slot 2(c-1)+1 for
+// The slots of the pieces of the unit (up to offset `unit_end` of its sequence)
+// that boundary c (at position `at`, offset `off`) is the first to cut, in key order: slot 2(c-1)+1 for
 // the unit's start, held by CTA c - 1, then 2c, 2(c+1), ... but for empty
 // pieces.  A thread takes a boundary.  Returns their number.
 constexpr uint32_t kMaxPieces = 600;
 template <int NT, class Where>
 __device__ uint32_t find_pieces(const BatchDev &b, uint32_t c, uint32_t C, const Pos &at, ull off, ull share,
-                                ull seqW, uint32_t nt, uint32_t *slots, Where where)
+                                ull unit_end, uint32_t nt, uint32_t *slots, Where where)
 {
     constexpr uint32_t kOut = 0xFFFFFFFFu;
     __shared__ uint32_t t_s[NT + 1];
@@ -293,7 +293,7 @@ __device__ uint32_t find_pieces(const BatchDev &b, uint32_t c, uint32_t C, const
         const uint32_t cc = c + k0 + threadIdx.x;          // a piece: boundaries cc and cc + 1
         const ull x = off + (ull)(k0 + threadIdx.x + 1) * share;
         uint32_t t = kOut;
-        if (cc + 1 < C && x < seqW) {
+        if (cc + 1 < C && x < unit_end) {
             const Pos nx = where(x);
             if (same_unit(nx, at)) t = nx.t;
         }
@@ -346,8 +346,8 @@ join_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint32_t pa
     key_tiles(g, s, at.rt, &first, &nt);
     ull base, slope;
     weights(g, s, &base, &slope);
-    const ull seqW = g.H * weight_before(base, slope, row_tiles(g, s));
-    const uint32_t K = find_pieces<NT>(b, c, sp.ctas, at, sh.off[1], quot(W + sp.ctas - 1, sp.ctas), seqW, nt,
+    const ull unit_end = at.h * weight_before(base, slope, row_tiles(g, s)) + weight_before(base, slope, at.rt + 1);
+    const uint32_t K = find_pieces<NT>(b, c, sp.ctas, at, sh.off[1], quot(W + sp.ctas - 1, sp.ctas), unit_end, nt,
                                        slots, [&](ull x) { return inside(g, s, at.i, x); });
     const uint32_t D = p.D, R = g.R, d4 = D / 4;
     const uint32_t live = min(R, (uint32_t)s.m * g.G - at.rt * R);

@@ -1101,7 +1101,8 @@ mass_join_kernel(MassGeo g, PagesDev p, BatchDev b, MassDev a, SplitDev sp)
     const SeqDev s = load_seq(b, p.bs.d, at.i);
     const MassSeq q = mass_seq(g, s);
     const uint32_t K = find_pieces<128>(b, c, sp.ctas, at, sh.off[1], quot(W + sp.ctas - 1, sp.ctas),
-                                        g.H * mass_before(g, s, q, q.kn), mass_tiles(g, s, q, at.rt), slots,
+                                        at.h * mass_before(g, s, q, q.kn) + mass_before(g, s, q, at.rt + 1),
+                                        mass_tiles(g, s, q, at.rt), slots,
                                         [&](ull x) { return mass_inside(g, s, at.i, x); });
     const uint32_t nb = kMK / p.bs.d, lb = threadIdx.x, gb = (q.kf + at.rt) * nb + lb;
     cudaGridDependencySynchronize();
