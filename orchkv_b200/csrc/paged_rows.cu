@@ -144,6 +144,7 @@ attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint
         const SeqDev s = load_seq(b, p.bs.d, at.i);
         const uint32_t RT = row_tiles(g, s);
         if (RT == 0) { at = Pos{at.i + 1, 0, 0, 0}; continue; }
+        if (at.i > end.i) break;                           // the end was a sequence without units
         const bool stop = same_unit(at, end);
         if (stop && end.t == 0) break;
         uint32_t first, nt;
@@ -675,7 +676,7 @@ template <class T, int DP, bool AL>
 int attend_a(const PagesDev &p, const BatchDev &b, const AttendDev &a, const ClassDev &cl,
              const SplitDev &sp, cudaStream_t s)
 {
-    const Geo g = {kR, kKeys, a.G, p.H, a.window, cl.min_rows, cl.max_rows};
+    const Geo g = {kR, kKeys, a.G, p.H, a.window, cl.min_rows, cl.max_rows, 0};
     if (sp.split) {
         auto k = attend_rows_kernel<T, DP, true, AL>;
         constexpr size_t smem = RowsCfg<DP>::smem + (size_t)kR * (DP + 2) * sizeof(float);
@@ -720,7 +721,7 @@ int attend_d(const PagesDev &p, const BatchDev &b, const AttendDev &a, const Cla
 template <class T, int DP>
 int mass_d(const PagesDev &p, const BatchDev &b, const MassDev &a, const ClassDev &cl, cudaStream_t s)
 {
-    const Geo g = {kR, 0, a.G, p.H, a.window, cl.min_rows, cl.max_rows};
+    const Geo g = {kR, 0, a.G, p.H, a.window, cl.min_rows, cl.max_rows, 0};
     const uint32_t per_item = p.bs.d >= 16 ? 1 : 16 / p.bs.d;
     const uint32_t items = (b.width + per_item - 1) / per_item;
     // A CTA takes 4 us to its first product (rows, queries, table, keys one

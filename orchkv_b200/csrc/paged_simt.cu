@@ -72,6 +72,7 @@ attend_simt_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp)
         const SeqDev s = load_seq(b, p.bs.d, at.i);
         const uint32_t RT = row_tiles(g, s);
         if (RT == 0) { at = Pos{at.i + 1, 0, 0, 0}; continue; }
+        if (at.i > end.i) break;                           // the end was a sequence without units
         if (same_unit(at, end) && end.t == 0) break;
         uint32_t first, nt;
         key_tiles(g, s, at.rt, &first, &nt);
@@ -288,7 +289,7 @@ template <class T>
 int attend(const PagesDev &p, const BatchDev &b, const AttendDev &a, const ClassDev &cl,
            const SplitDev &sp, cudaStream_t s)
 {
-    const Geo g = {kSimtRows, kSimtKeys, a.G, p.H, a.window, cl.min_rows, cl.max_rows};
+    const Geo g = {kSimtRows, kSimtKeys, a.G, p.H, a.window, cl.min_rows, cl.max_rows, 0};
     attend_simt_kernel<T><<<sp.ctas, kW * 32, 0, s>>>(g, p, b, a, sp);
     note_launches(1);
     OKV_CUDA_TRY(cudaGetLastError());
@@ -302,7 +303,7 @@ int attend(const PagesDev &p, const BatchDev &b, const AttendDev &a, const Class
 template <class T>
 int mass(const PagesDev &p, const BatchDev &b, const MassDev &a, const ClassDev &cl, cudaStream_t s)
 {
-    const Geo g = {kSimtRows, kSimtKeys, a.G, p.H, a.window, cl.min_rows, cl.max_rows};
+    const Geo g = {kSimtRows, kSimtKeys, a.G, p.H, a.window, cl.min_rows, cl.max_rows, 0};
     const uint32_t per_warp = p.bs.d >= 32 ? 1 : 32 / p.bs.d;
     const uint32_t groups = (b.width + kW * per_warp - 1) / (kW * per_warp);
     const unsigned long long grid = (unsigned long long)b.n * p.H * groups;

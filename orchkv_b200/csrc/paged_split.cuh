@@ -32,6 +32,7 @@ __device__ __forceinline__ ull quot(ull x, ull y)
 struct Geo {                     // what the division depends on besides the lengths
     uint32_t R, KT, G, H, window;
     uint32_t min_rows, max_rows;
+    uint32_t join;               // what a join costs, in keys of a unit
 };
 
 __device__ __forceinline__ uint32_t row_tiles(const Geo &g, const SeqDev &s)
@@ -76,8 +77,11 @@ struct Pos {
     uint32_t i, h, rt, t;        // t counts from the unit's first key tile; i == n: the end
 };
 
-// Position of offset x inside sequence i's weight.
-__device__ __forceinline__ Pos inside(const Geo &g, const SeqDev &s, uint32_t i, ull x)
+// Position of offset x inside sequence i's weight.  A unit is cut only if that
+// gains more than the join costs: not when whole units leave a CTA (of `share`)
+// at most g.join keys more to do; the boundary then goes to the unit's nearer
+// end.
+__device__ __forceinline__ Pos inside(const Geo &g, const SeqDev &s, uint32_t i, ull x, ull share)
 {
     ull base, slope;
     weights(g, s, &base, &slope);
@@ -103,6 +107,17 @@ __device__ __forceinline__ Pos inside(const Geo &g, const SeqDev &s, uint32_t i,
     uint32_t first, nt;
     key_tiles(g, s, p.rt, &first, &nt);
     const ull z = y - weight_before(base, slope, rt), w = base + slope * rt;
+    if (quot(share + w - 1, w) * w <= share + (ull)g.join * g.G) {
+        p.t = 0;
+        if (2 * z >= w && ++p.rt == RT) {
+            p.rt = 0;
+            if (++p.h == g.H) {
+                p.h = 0;
+                p.i++;                   // a sequence without units, or the end, perhaps
+            }
+        }
+        return p;
+    }
     p.t = (uint32_t)quot(z * nt, w);
     return p;
 }
@@ -150,7 +165,7 @@ template <int NT> __device__ __forceinline__ ull block_scan(ull v, ull *red, ull
 
 // Boundaries c and c + 1 of C equal shares, by the whole block; *total 0: no
 // work.  The end of the list is {n, 0, 0, 0}.  weight(i) is sequence i's part
-// of the list, where(s, i, x) the position of offset x in it.
+// of the list, where(s, i, x, share) the position of offset x in it.
 template <int NT, class Weight, class Where>
 __device__ void find_share(const BatchDev &b, uint32_t bs, uint32_t c, uint32_t C, SplitShared *sh, Pos *from,
                            Pos *to, ull *W, Weight weight, Where where)
@@ -177,7 +192,7 @@ __device__ void find_share(const BatchDev &b, uint32_t bs, uint32_t c, uint32_t 
             const uint32_t i = in ? __ffs(in) - 1 : 0;
             const ull off = x - __shfl_sync(0xFFFFFFFFu, inc - w, i);
             if (k == 1 && threadIdx.x == 0) sh->off[1] = off;
-            *out[k] = in ? where(load_seq(b, bs, i), i, off) : Pos{b.n, 0, 0, 0};
+            *out[k] = in ? where(load_seq(b, bs, i), i, off, share) : Pos{b.n, 0, 0, 0};
         }
         return;
     }
@@ -223,7 +238,7 @@ __device__ void find_share(const BatchDev &b, uint32_t bs, uint32_t c, uint32_t 
     for (int k = 0; k < 2; k++) {
         const uint32_t i = sh->seq[k];
         if (i >= b.n) *out[k] = Pos{b.n, 0, 0, 0};
-        else *out[k] = where(load_seq(b, bs, i), i, sh->off[k]);
+        else *out[k] = where(load_seq(b, bs, i), i, sh->off[k], share);
     }
     __syncthreads();
 }
@@ -232,7 +247,7 @@ __device__ void find_share(const Geo &g, const BatchDev &b, uint32_t bs, uint32_
                            SplitShared *sh, Pos *from, Pos *to, ull *W)
 {
     find_share<NT>(b, bs, c, C, sh, from, to, W, [&](uint32_t i) { return seq_weight(g, b, bs, i); },
-                   [&](const SeqDev &s, uint32_t i, ull x) { return inside(g, s, i, x); });
+                   [&](const SeqDev &s, uint32_t i, ull x, ull share) { return inside(g, s, i, x, share); });
 }
 
 __device__ __forceinline__ bool same_unit(const Pos &a, const Pos &b)
@@ -347,8 +362,9 @@ join_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint32_t pa
     ull base, slope;
     weights(g, s, &base, &slope);
     const ull unit_end = at.h * weight_before(base, slope, row_tiles(g, s)) + weight_before(base, slope, at.rt + 1);
-    const uint32_t K = find_pieces<NT>(b, c, sp.ctas, at, sh.off[1], quot(W + sp.ctas - 1, sp.ctas), unit_end, nt,
-                                       slots, [&](ull x) { return inside(g, s, at.i, x); });
+    const ull share = quot(W + sp.ctas - 1, sp.ctas);
+    const uint32_t K = find_pieces<NT>(b, c, sp.ctas, at, sh.off[1], share, unit_end, nt, slots,
+                                       [&](ull x) { return inside(g, s, at.i, x, share); });
     const uint32_t D = p.D, R = g.R, d4 = D / 4;
     const uint32_t live = min(R, (uint32_t)s.m * g.G - at.rt * R);
     const uint32_t each = (live + parts - 1) / parts, r_end = min(live, (part + 1) * each);

@@ -46,6 +46,10 @@ constexpr uint32_t kR = 256, kK = 128;
 // half 1 (64, 128 and 64 columns), then O of either half.
 constexpr uint32_t kP0 = 0, kS = 64, kP1 = 192;
 constexpr float kGrow = 8.f;               // log2 of the growth that O is scaled at
+// A join costs 20 to 30 us (every cut unit's partials are 128 KB written and read),
+// as long as 10 tiles of keys: 512 tokens over 1000, 32/8 heads: 68 us with every
+// boundary cut, 48 with none.
+constexpr uint32_t kJoinKeys = 10 * kK;
 constexpr int kMeta = 8;                   // tiles whose column masks are kept
 
 template <int DP> struct TileCfg {
@@ -561,14 +565,16 @@ template <class T, int DP>
 int go(const CUtensorMap &km, const CUtensorMap &vm, const PagesDev &p, const BatchDev &b, const AttendDev &a,
        const ClassDev &cl, const SplitDev &sp, cudaStream_t s)
 {
-    const Geo g = {kR, kK, a.G, p.H, a.window, cl.min_rows, cl.max_rows};
+    const Geo g = {kR, kK, a.G, p.H, a.window, cl.min_rows, cl.max_rows, kJoinKeys};
     auto k = attend_tile_kernel<T, DP>;
     static std::atomic<uint64_t> done;
     OKV_CUDA_TRY(allow_smem(k, TileCfg<DP>::smem, done));
     k<<<sp.ctas, kThreads, TileCfg<DP>::smem, s>>>(km, vm, g, p, b, a, sp, p.head_b == 0);
     note_launches(1);
     OKV_CUDA_TRY(cudaGetLastError());
-    if (sp.ctas > 1) {
+    // units of at most so many keys are never cut
+    const unsigned long long most = (unsigned long long)b.width * p.bs.d + 64 + kR;
+    if (sp.ctas > 1 && most > kJoinKeys) {
         OKV_CUDA_TRY(launch_after(join_kernel<T, 256>, (sp.ctas - 1) * 8, 256, 0, s, g, p, b, a, sp, 8u));
         note_launches(1);
     }
@@ -773,7 +779,7 @@ mass_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     ull W;
     find_share<kMassThreads>(b, p.bs.d, blockIdx.x, sp.ctas, &sh.split, &w.at, &w.end, &W,
                              [&](uint32_t i) { return mass_weight(g, b, p.bs.d, i); },
-                             [&](const SeqDev &s, uint32_t i, ull x) { return mass_inside(g, s, i, x); });
+                             [&](const SeqDev &s, uint32_t i, ull x, ull) { return mass_inside(g, s, i, x); });
     cudaTriggerProgrammaticLaunchCompletion();
     if (W == 0) return;
     if (!w.settle()) return;
@@ -1091,7 +1097,7 @@ mass_join_kernel(MassGeo g, PagesDev p, BatchDev b, MassDev a, SplitDev sp)
     ull W;
     find_share<128>(b, p.bs.d, c - 1, sp.ctas, &sh, &prev, &at, &W,
                     [&](uint32_t i) { return mass_weight(g, b, p.bs.d, i); },
-                    [&](const SeqDev &s, uint32_t i, ull x) { return mass_inside(g, s, i, x); });
+                    [&](const SeqDev &s, uint32_t i, ull x, ull) { return mass_inside(g, s, i, x); });
     // (no block ends before the kernel in front: the next launch counts on that)
     if (W == 0 || at.i >= b.n || at.t == 0 || (same_unit(prev, at) && prev.t > 0)) {
         cudaGridDependencySynchronize();

@@ -281,6 +281,7 @@ struct Walk {
             s = load_seq(b, bs, at.i);
             RT = row_tiles(g, s);
             if (RT == 0) { at = Pos{at.i + 1, 0, 0, 0}; continue; }
+            if (at.i > end.i) return false;            // the end was a sequence without units
             stop = same_unit(at, end);
             key_tiles(g, s, at.rt, &first, &nt);
             t0 = at.t;
