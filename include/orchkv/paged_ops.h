@@ -29,7 +29,7 @@ extern "C" {
 
 /* The pages.  Element (page p, KV head h, token t, d) of K is at
  * k[p * page_stride + h * head_stride + t * token_stride + d], strides in
- * elements, V alike.  The data plane's slabs are pages of one head: k =
+ * elements and not negative, V alike.  The data plane's slabs are pages of one head: k =
  * orchkv_gpu_pool_base(), v = k + half a slab, head_stride 0, page_stride
  * one slab.  k, v and every stride must be multiples of 16 bytes; d_head a
  * multiple of 16 bytes, at most 256 elements. */
@@ -109,6 +109,7 @@ typedef struct orchkv_attend_args {
  * What lies in places that a row does not attend to does not reach it, be it
  * infinite or NaN; an infinite or NaN value reaches every row that does, as
  * such or as NaN.
+ * out must not overlap q.
  * workspace: orchkv_paged_attend_workspace() bytes of device memory, 256-byte
  * aligned, of this call alone until it has run.  Asynchronous. */
 size_t orchkv_paged_attend_workspace(const orchkv_pages_t *pages, const orchkv_batch_t *batch,

@@ -14,7 +14,8 @@ constexpr uint64_t kMaxTokens = 1ull << 30;      // of one sequence's table
 
 bool aligned(const void *p, int64_t s0, int64_t s1, size_t e)
 {
-    return p && (uintptr_t)p % 16 == 0 && (s0 * (int64_t)e) % 16 == 0 && (s1 * (int64_t)e) % 16 == 0;
+    return p && (uintptr_t)p % 16 == 0 && s0 >= 0 && s1 >= 0 && (s0 * (int64_t)e) % 16 == 0 &&
+           (s1 * (int64_t)e) % 16 == 0;
 }
 
 bool rows_ok(const orchkv_rows_t &r, size_t e) { return aligned(r.p, r.row_stride, r.head_stride, e); }
@@ -28,7 +29,8 @@ bool shapes_ok(const orchkv_pages_t *p, const orchkv_batch_t *b, bool need_v)
     if (p->page_tokens == 0 || p->n_kv_heads == 0 || p->n_kv_heads > 65535 || p->n_pages == 0 ||
         p->n_pages > 0x7FFFFFFFu)
         return false;
-    if (!aligned(p->k, p->page_stride, p->head_stride, e) || (p->token_stride * (int64_t)e) % 16)
+    if (!aligned(p->k, p->page_stride, p->head_stride, e) || p->token_stride < 0 ||
+        (p->token_stride * (int64_t)e) % 16)
         return false;
     if (need_v && !aligned(p->v, 0, 0, e)) return false;
     if (b->n_seqs && (!b->table || !b->lens || !b->starts)) return false;
@@ -100,6 +102,9 @@ bool small_call(const orchkv_pages_t *p, const orchkv_batch_t *b, uint64_t G, ui
 }
 
 // What one attend call launches, from what the host knows of it.
+// No sequence is longer than 2^30: a larger window is no window.
+uint32_t window_of(uint32_t w) { return w > (1u << 30) ? 0 : w; }
+
 struct AttendPlan {
     SplitDev rows, tile;     // ctas 0: not launched
     ClassDev few, many;
@@ -213,7 +218,8 @@ int orchkv_paged_attend(const orchkv_pages_t *pages, const orchkv_batch_t *batch
         return ORCHKV_ERR_INVALID;
     if (batch->n_rows == 0 || batch->n_seqs == 0) return ORCHKV_OK;
     const size_t e = dtype_size((DataType)pages->dtype);
-    if (!rows_ok(args->q, e) || !rows_ok(args->out, e)) return ORCHKV_ERR_INVALID;
+    // (several CTAs read a row of q that one of them writes the result of)
+    if (!rows_ok(args->q, e) || !rows_ok(args->out, e) || args->q.p == args->out.p) return ORCHKV_ERR_INVALID;
     AttendPlan pl = plan_attend(pages, batch, args);
     if (pl.bytes && (!workspace || (uintptr_t)workspace % 256 || bytes < pl.bytes)) return ORCHKV_ERR_INVALID;
     AttendDev a;
@@ -222,7 +228,7 @@ int orchkv_paged_attend(const orchkv_pages_t *pages, const orchkv_batch_t *batch
     a.lse = args->lse;
     a.Hq = args->n_q_heads;
     a.G = args->n_q_heads / pages->n_kv_heads;
-    a.window = args->window;
+    a.window = window_of(args->window);
     a.sl2 = args->scale * 1.4426950408889634f;
     const PagesDev p = pages_dev(pages);
     const BatchDev b = batch_dev(batch);
@@ -260,7 +266,7 @@ int orchkv_paged_block_mass(const orchkv_pages_t *pages, const orchkv_batch_t *b
     a.mass = args->mass;
     a.Hq = args->n_q_heads;
     a.G = args->n_q_heads / pages->n_kv_heads;
-    a.window = args->window;
+    a.window = window_of(args->window);
     a.sl2 = args->scale * 1.4426950408889634f;
     const PagesDev p = pages_dev(pages);
     const BatchDev b = batch_dev(batch);

@@ -1191,7 +1191,7 @@ bool rows_map(CUtensorMap *m, const RowsDev &q, uint32_t D, uint32_t Hq, uint32_
 // the scores (the mask is applied before it).
 bool attend_tile_takes(const PagesDev &p, int dtype, float sl2)
 {
-    return dtype != DTYPE_FP32 && pages_tile(p) && sl2 > 0.f && p.page_b >= 0 && p.head_b >= 0 && p.tok_b > 0 &&
+    return dtype != DTYPE_FP32 && pages_tile(p) && sl2 > 0.f && p.page_b > 0 && p.tok_b > 0 &&
            p.page_b < (1ll << 40) && p.head_b < (1ll << 40) && p.tok_b < (1ll << 40);
 }
 

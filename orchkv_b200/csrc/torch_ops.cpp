@@ -105,6 +105,7 @@ public:
         c10::cuda::CUDAGuard guard(dev_);
         if (!out) out = at::empty(q.sizes(), q.options());
         a.out = row_tensor(*out, "out", hq, rows);
+        if (rows && a.out.p == a.q.p) refuse("out must not overlap q");
         Tensor lse;
         if (return_lse) {
             lse = at::empty({rows, hq}, q.options().dtype(at::kFloat));

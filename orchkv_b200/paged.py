@@ -214,7 +214,7 @@ class PagedKV:
         """softmax(scale * q k) v of every row of q [rows, query heads,
         head_dim] over its sequence's tokens up to its own place (the last
         `window` of them if not 0); scale is head_dim ** -0.5 by default.
-        Returns out, or (out, lse) with lse [rows, query heads] fp32.  A row
+        Returns out (not q), or (out, lse) with lse [rows, query heads] fp32.  A row
         with nothing to attend to gets 0 and -inf.  max_new: the most new
         tokens of one sequence, if the caller knows it (decode: 1), lets the
         call leave out what only longer ones need; the rows of a sequence

@@ -483,6 +483,7 @@ def test_refusals(cuda):
         (lambda: x.attend(c["q"], *a, window=-1), "window"),
         (lambda: x.attend(c["q"], *a, max_new=-1), "max_new"),
         (lambda: x.attend(c["q"], *a, out=c["q"][:2]), "out must be"),
+        (lambda: x.attend(c["q"], *a, out=c["q"]), "overlap"),
         (lambda: x.attend(c["q"].float().requires_grad_().to(c["dt"]), *a), "gradient"),
         (lambda: x.append(c["k"][:2], c["v"], *a), "v must be"),
         (lambda: x.append(c["q"], c["v"], *a), "k must be"),

@@ -18,7 +18,7 @@ def call(**kw):
     """A valid call's arguments, by name, with some replaced."""
     v = dict(k=A, v=A, page_stride=16 * 4 * 128, head_stride=128, token_stride=4 * 128, n_pages=9,
              page_tokens=16, n_kv_heads=4, d_head=128, dtype=1, table=A, width=4096, n=2, lens=A, starts=A,
-             rows=6, hq=8, q=A, out=A, row_stride=8 * 128, q_head=128, kr=A, vr=A, rot=128, turns=A,
+             rows=6, hq=8, q=A, out=2 * A, row_stride=8 * 128, q_head=128, kr=A, vr=A, rot=128, turns=A,
              ws=A, short=0)
     assert set(kw) <= set(v)
     v.update(kw)
@@ -54,6 +54,8 @@ EVERY = ("append", "attend", "mass")
     (dict(hq=0), ("attend", "mass")), (dict(q=0), EVERY), (dict(q=A + 2), EVERY), (dict(out=0), EVERY),
     (dict(row_stride=8 * 128 + 1), EVERY), (dict(q_head=129), EVERY), (dict(kr=0), ("append",)),
     (dict(vr=A + 8), ("append",)), (dict(rot=127), ("append",)), (dict(rot=130), ("append",)),
+    (dict(page_stride=-16 * 4 * 128), EVERY), (dict(token_stride=-128), EVERY), (dict(row_stride=-1024), EVERY),
+    (dict(out=A), ("attend",)),
     (dict(turns=0), ("append",)), (dict(ws=0), ("attend",)), (dict(ws=A + 16), ("attend",)),
     (dict(short=1), ("attend",)),
 ])
