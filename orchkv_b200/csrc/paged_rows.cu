@@ -14,9 +14,9 @@
 // CTAs' as paged_split.cuh describes.  Places outside the range of every row,
 // past the length or in no page are filled with zeros and never read.
 //
-// 32 requests x 1 token over 8192, 28/4 heads of 128, bf16: 96 us, 5.6 TB/s,
-// 0.85 of the measured copy rate, 89 of them this kernel and 6 the join; 61
-// requests over 1 to 16000 tokens, window 6000: 208 us, 0.91.
+// 32 requests x 1 token over 8192, 28/4 heads of 128, bf16: 96 to 101 us over the
+// boxes measured, 0.81 to 0.85 of the measured copy rate, 6 us of them the join;
+// 61 requests over 1 to 16000 tokens, window 6000: 208 us, 0.91.
 #include <algorithm>
 
 #include "kernels.h"
@@ -64,7 +64,9 @@ __device__ __forceinline__ void cluster_meet()
 
 // Before a product with 16 keys that only some rows attend to: a weight of 0
 // times an infinite or NaN value would reach the rows that do not, so such
-// values become 0 and the results of the rows that do attend NaN.
+// values become 0 and the results of the rows that do attend NaN.  Only groups
+// on a chunk's diagonal or a window's edge come here (1.5 % of a decode step
+// that never does, by its registers).
 template <class T, int DP>
 __device__ __forceinline__ void drop_infinite(uint32_t vt, const RowInfo &r0, const RowInfo &r1, int k0,
                                               uint32_t have, float (*acc)[4])
