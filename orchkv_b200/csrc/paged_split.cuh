@@ -42,18 +42,25 @@ __device__ __forceinline__ uint32_t row_tiles(const Geo &g, const SeqDev &s)
 }
 
 // Weight of row tile rt: base + slope * rt, in keys * G; 64 keys' worth stand
-// for a unit's fixed cost.
+// for a unit's fixed cost.  Where the rows' places are not those of the tokens
+// in the table (lens says more tokens than the table holds, or fewer than the
+// rows), every row tile counts as if it read them all.  So no unit weighs more
+// than G * (keys of the table + 64) + R, which may_cut goes by.
 __device__ __forceinline__ void weights(const Geo &g, const SeqDev &s, ull *base, ull *slope)
 {
-    const uint32_t c0 = s.c0 > 0 ? s.c0 : 0;
-    if (g.window && g.window < c0 + s.m) {
+    const bool odd = s.c0 < 0 || s.c0 + s.m > s.len;
+    const uint32_t keys = odd ? s.len : s.c0;
+    if (g.window && g.window < keys + (odd ? 0 : s.m)) {
         *base = (ull)g.G * (g.window + 64) + g.R;
         *slope = 0;
     } else {
-        *base = (ull)g.G * (c0 + 64) + g.R;
-        *slope = g.R;
+        *base = (ull)g.G * (keys + 64) + g.R;
+        *slope = odd ? 0 : g.R;
     }
 }
+// Units over tables of at most so many keys are never cut: whole units leave a
+// CTA less than the heaviest one over its share, so at most g.join keys over.
+inline bool may_cut(const Geo &g, ull keys) { return keys + 64 + g.R > g.join; }
 __device__ __forceinline__ ull weight_before(ull base, ull slope, ull rt)
 {
     return rt * base + slope * (rt * (rt - 1) / 2 * (rt > 0));

@@ -573,9 +573,7 @@ int go(const CUtensorMap &km, const CUtensorMap &vm, const PagesDev &p, const Ba
     k<<<sp.ctas, kThreads, TileCfg<DP>::smem, s>>>(km, vm, g, p, b, a, sp, p.head_b == 0);
     note_launches(1);
     OKV_CUDA_TRY(cudaGetLastError());
-    // units of at most so many keys are never cut
-    const unsigned long long most = (unsigned long long)b.width * p.bs.d + 64 + kR;
-    if (sp.ctas > 1 && most > kJoinKeys) {
+    if (sp.ctas > 1 && may_cut(g, (ull)b.width * p.bs.d)) {
         OKV_CUDA_TRY(launch_after(join_kernel<T, 256>, (sp.ctas - 1) * 8, 256, 0, s, g, p, b, a, sp, 8u));
         note_launches(1);
     }

@@ -1,0 +1,55 @@
+"""The paged operators where lengths, values and memory are unusual: lengths
+past the table, infinities and NaN, faint weights, gradients, overlapping
+tensors.  Bounds are those of tests/paged_cases.py."""
+import math
+
+import pytest
+
+from oracle import paged_model as M
+from tests import paged_cases as P
+
+pytestmark = pytest.mark.gpu
+
+
+def kv(c):
+    from orchkv_b200 import paged
+    return paged.PagedKV(c["kp"], c["vp"], c["layout"])
+
+
+def call(c):
+    return c["table"], c["lens"], c["starts"]
+
+
+# ---- lengths that the table does not cover -----------------------------------------
+
+def past_the_table(torch, new, lens, tokens, **kw):
+    """Sequences of new[i] rows and lens[i] tokens over tables of `tokens`, of
+    which the first min(lens[i], tokens) lie in pages."""
+    there = [min(n, tokens) for n in lens]
+    c = P.make(torch, [0] * len(new), there, width=tokens // kw.get("block", 16), **kw)
+    c["lens"] = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    c["starts"] = torch.tensor([sum(new[:i]) for i in range(len(new) + 1)], dtype=torch.int32, device="cuda")
+    hq, d = c["q"].shape[1:]
+    c["q"] = torch.randn(sum(new), hq, d, generator=c["gen"], device="cuda").to(c["dt"])
+    return c
+
+
+@pytest.mark.parametrize("new,lens,tokens,hq,hk", [
+    ([2048], [3000], 960, 32, 8), ([2048], [9000], 960, 32, 8), ([3000], [900], 960, 8, 1),
+    ([1500, 70], [2500, 4000], 960, 16, 4), ([1200, 900], [1000, 5000], 960, 8, 1), ([2000], [5000], 4000, 8, 2),
+    ([1, 1, 1], [500, 2000, 9000], 960, 8, 2), ([5, 3], [2, 3000], 960, 8, 2),
+])
+@pytest.mark.parametrize("window", [0, 700])
+def test_lengths_past_the_table_or_below_the_rows(cuda, new, lens, tokens, hq, hk, window):
+    """Every row is written: tokens past the table hold nothing, and rows
+    before a sequence's first token attend to nothing."""
+    torch = cuda
+    d = 64
+    c = past_the_table(torch, new, lens, tokens, hq=hq, hk=hk, d=d, seed=sum(new))
+    out = torch.full_like(c["q"], 7.0)
+    got, lse = kv(c).attend(c["q"], *call(c), window=window, return_lse=True, out=out)
+    assert got is out
+    P.check_attend(c, out, lse, d ** -0.5, window)
+    mass = torch.full((len(new), hk, tokens // 16), 7.0, device="cuda")
+    kv(c).block_mass(c["q"], lse, *call(c), window=window, out=mass)
+    P.check_mass(c, mass, lse, d ** -0.5, window)
