@@ -69,6 +69,17 @@ __device__ __forceinline__ float ex2(float x)
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
+// Log2 of what the weights of the second product are multiplied with.  They
+// are rounded to the pages' type, half a step each; of fp16 that holds down to
+// 2^-14 only, so the largest weight (2^grow times the reference) is 2^15
+// there: weights down to 2^(grow - 29) of the largest keep their 11 bits, and
+// smaller ones are off by 2^(grow - 40) of it at most.  The maximum and the sum
+// that go with the weights are taken with it, so results do not see it.
+template <class T> __host__ __device__ constexpr float weight_bias(float grow)
+{
+    return std::is_same<T, __half>::value ? 15.f - grow : 0.f;
+}
+
 // Whether 16-bit values are all finite, a pair at a time: x * 0 is 0 for a finite
 // x and NaN for the others, and stays NaN in a sum.
 template <class T> struct Finite;

@@ -247,7 +247,7 @@ attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint
                                          fmaxf(sc[1][2 * x], sc[1][2 * x + 1]));
                         mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
                         mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
-                        mx = fmaxf(mx, m[x]);
+                        mx = fmaxf(mx - weight_bias<T>(0.f), m[x]);
                         const float ms = mx == -INFINITY ? 0.f : mx;
                         f[x] = ex2(m[x] - ms);
                         m[x] = mx;
@@ -255,8 +255,8 @@ attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint
 #pragma unroll
                         for (int j = 0; j < 4; j++) q[j] = ex2(sc[j >> 1][2 * x + (j & 1)] - ms);
                         l[x] = l[x] * f[x] + ((q[0] + q[1]) + (q[2] + q[3]));
-                        // the weights are rounded to the pages' type (they are
-                        // at most 1): half a step each, as the result's own
+                        // the weights are rounded to the pages' type: half a
+                        // step each, as the result's own (see weight_bias)
                         pf[x] = pack2<T>(q[0], q[1]);
                         pf[2 + x] = pack2<T>(q[2], q[3]);
                     }

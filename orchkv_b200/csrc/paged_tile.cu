@@ -16,8 +16,8 @@
 // weights never touch shared memory) and one S of 128 that the halves fill and
 // read in turn: a half's next scores are computed while it still weighs its
 // last ones.  O stays there; it is scaled only when a row's maximum has grown
-// by more than 2^8 (weights then reach 256, which neither type nor the fp32
-// sums mind), which after the first tiles is rare.
+// by more than 2^8 (fp16: 2^4; the weights in between are larger than 1, which
+// neither type nor the fp32 sums mind), which after the first tiles is rare.
 //
 // 4096 new tokens over 28672, 32/8 heads of 128, bf16: 1.77 to 2.01 ms over the
 // boxes measured, 1030 to 1170 TFLOP/s, 0.62 to 0.71 of the measured matrix rate
@@ -46,7 +46,9 @@ constexpr uint32_t kR = 256, kK = 128;
 // Columns of tensor memory: the weights of half 0, the scores, the weights of
 // half 1 (64, 128 and 64 columns), then O of either half.
 constexpr uint32_t kP0 = 0, kS = 64, kP1 = 192;
-constexpr float kGrow = 8.f;               // log2 of the growth that O is scaled at
+// Log2 of the growth that O is scaled at: less for fp16, whose weights have
+// less room above and below.
+template <class T> constexpr float kGrow = std::is_same<T, __half>::value ? 4.f : 8.f;
 // A join costs 20 to 30 us (every cut unit's partials are 128 KB written and read),
 // as long as 10 tiles of keys: 512 tokens over 1000, 32/8 heads: 68 us with every
 // boundary cut, 48 with none.
@@ -414,7 +416,8 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
 #pragma unroll
                     for (int k = 0; k < 4; k++) mx[k] = max3(mx[k], s[j + k], s[j + k + 4]);
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                const float ms = top * a.sl2;          // the scale is positive here
+                // the scale is positive here
+                const float ms = fmaf(top, a.sl2, -weight_bias<T>(kGrow<T>));
                 if (t == w.t0) {
                     m = ms;
                 } else {
@@ -424,7 +427,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                     if (!ok) break;
                     o_ph ^= 1;
                     tm_after();
-                    const bool grow = ms > m + kGrow || (m == -INFINITY && ms > m);
+                    const bool grow = ms > m + kGrow<T> || (m == -INFINITY && ms > m);
                     if (__any_sync(0xFFFFFFFFu, grow)) {
                         const float nm = grow ? ms : m;
                         const float f = nm == -INFINITY ? 1.f : ex2(m - nm);

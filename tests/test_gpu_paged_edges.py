@@ -53,3 +53,46 @@ def test_lengths_past_the_table_or_below_the_rows(cuda, new, lens, tokens, hq, h
     mass = torch.full((len(new), hk, tokens // 16), 7.0, device="cuda")
     kv(c).block_mass(c["q"], lse, *call(c), window=window, out=mass)
     P.check_mass(c, mass, lse, d ** -0.5, window)
+
+
+# ---- faint weights --------------------------------------------------------------------
+
+@pytest.mark.parametrize("new,held,block", [([1], 32000, 16), ([40], 32000, 16), ([600], 32000, 16),
+                                            ([40], 32000, 24), ([1] * 48, 6000, 16)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("where", ["first", "last"])
+def test_one_large_weight_among_many_faint_ones(cuda, new, held, block, d, dtype, where):
+    """One key of weight 1 whose value is 0, and thousands of weight e^-17 =
+    2^-24.5: the result is theirs alone, so each must be held to half a step
+    of the pages' type."""
+    torch = cuda
+    c = P.make(torch, new, [held] * len(new), hq=8, hk=2, d=d, block=block, dtype=dtype, stale=0.0)
+    c["kp"].zero_()
+    c["q"].zero_()
+    c["q"][:, :, 0] = 4.0
+    at = 0 if where == "first" else held - 1
+    page = c["table"][:, at // block].long()
+    c["kp"][page, at % block, :, 0] = 4.25
+    c["vp"].copy_(1 + 0.25 * torch.rand(c["vp"].shape, generator=c["gen"], device="cuda"))
+    c["vp"][page, at % block] = 0
+    out, lse = kv(c).attend(c["q"], *call(c), scale=1.0, return_lse=True)
+    P.check_attend(c, out, lse, 1.0)
+
+
+@pytest.mark.parametrize("new", [1, 40, 600])
+@pytest.mark.parametrize("rise", [0.5, 2.0, 3.5, 6.0])
+def test_scores_that_rise_along_the_keys(cuda, new, rise):
+    """Scores that grow by `rise` nats every 128 keys: the reference that
+    weights are taken against lags behind or is moved, and fp16 holds both."""
+    torch = cuda
+    c = P.make(torch, [new], [2000], hq=8, hk=2, d=64, dtype="fp16", stale=0.0)
+    c["q"].zero_()
+    c["q"][:, :, 0] = 1.0
+    tok = torch.arange(2000 + new, device="cuda")
+    row = c["table"][0, tok // 16].long()
+    c["kp"].mul_(0.25)
+    c["kp"][row, tok % 16, :, 0] = (rise * (tok // 128)).to(c["dt"])[:, None]
+    out, lse = kv(c).attend(c["q"], *call(c), scale=1.0, return_lse=True)
+    assert torch.isfinite(out).all()
+    P.check_attend(c, out, lse, 1.0)
