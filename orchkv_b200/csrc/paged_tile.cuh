@@ -206,18 +206,31 @@ __device__ __forceinline__ ull mul2(ull a, ull b)
     return r;
 }
 
-// Two powers of two without the special function unit, for arguments below
-// 2^7: x = n + f with |f| <= 1/2 (adding 1.5 * 2^23 rounds x to n and leaves n
-// in the low bits), 2^f by a polynomial, n into the exponent.  Arguments below
-// -126 count as -126.  The polynomial of degree 5 minimises the largest
-// relative error over [-1/2, 1/2] (Remez exchange in double, coefficients
-// rounded): 2.1e-7 when evaluated in fp32, 5e-8 on average, about what a sum
-// of many is off by.
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float min_nan(float a, float b)
+{
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// Two powers of two without the special function unit: x = n + f with |f| <=
+// 1/2 (adding 1.5 * 2^23 rounds x to n and leaves n in the low bits), 2^f by a
+// polynomial, times 2^n.  Arguments are held to [-127, 128], where the bits of
+// 2^n are those of 0 and of infinity; NaN stays NaN.  The polynomial of degree
+// 5 minimises the largest relative error over [-1/2, 1/2] (Remez exchange in
+// double, coefficients rounded): 2.1e-7 when evaluated in fp32, 5e-8 on
+// average, about what a sum of many is off by.
 __device__ __forceinline__ ull ex2_poly(ull x)
 {
     float a, b;
     unf2(x, &a, &b);
-    x = f2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+    x = f2(min_nan(max_nan(a, -127.f), 128.f), min_nan(max_nan(b, -127.f), 128.f));
     const ull t = add2(x, f2(12582912.f, 12582912.f));
     const ull f = fma2(add2(t, f2(-12582912.f, -12582912.f)), f2(-1.f, -1.f), x);
     constexpr float c[6] = {0x1.000002p+0f, 0x1.62e428p-1f, 0x1.ebf918p-3f, 0x1.c6b6e4p-5f, 0x1.3d0c52p-7f,
@@ -225,11 +238,9 @@ __device__ __forceinline__ ull ex2_poly(ull x)
     ull p = f2(c[5], c[5]);
 #pragma unroll
     for (int k = 4; k >= 0; k--) p = fma2(p, f, f2(c[k], c[k]));
-    float ta, tb;
-    unf2(t, &ta, &tb);
-    unf2(p, &a, &b);
-    return f2(__uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23)),
-              __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23)));
+    unf2(t, &a, &b);
+    return mul2(p, f2(__uint_as_float((__float_as_uint(a) << 23) + 0x3F800000u),
+                      __uint_as_float((__float_as_uint(b) << 23) + 0x3F800000u)));
 }
 
 __device__ __forceinline__ void tma3(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar)

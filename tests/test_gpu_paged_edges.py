@@ -96,3 +96,58 @@ def test_scores_that_rise_along_the_keys(cuda, new, rise):
     out, lse = kv(c).attend(c["q"], *call(c), scale=1.0, return_lse=True)
     assert torch.isfinite(out).all()
     P.check_attend(c, out, lse, 1.0)
+
+
+# ---- masses of values that are not finite --------------------------------------------
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("fp16", 64)])
+@pytest.mark.parametrize("of", ["q", "lse"])
+def test_a_nan_row_reaches_every_block_it_attends_to(cuda, dtype, d, of):
+    """A NaN query or lse in every place of a tile of 128 rows: all blocks
+    that the row attends to, and those of its KV head alone."""
+    torch = cuda
+    c = P.make(torch, [64], [512], hq=8, hk=2, d=d, dtype=dtype)
+    _, lse = kv(c).attend(c["q"], *call(c), return_lse=True)
+    clean = kv(c).block_mass(c["q"], lse, *call(c))
+    P.check_mass(c, clean, lse, d ** -0.5)
+    for col in range(128):
+        row, g = col // 4 + 32 * (col & 1), col % 4
+        h = col // 64
+        q, l = c["q"].clone(), lse.clone()
+        if of == "q":
+            q[row, h * 4 + g, col % d] = math.nan
+        else:
+            l[row, h * 4 + g] = math.nan
+        mass = kv(c).block_mass(q, l, *call(c))
+        blocks = (512 + row) // 16 + 1
+        assert torch.isnan(mass[0, h, :blocks]).all(), col
+        assert torch.equal(mass[0, h, blocks:], clean[0, h, blocks:]), col
+        assert torch.equal(mass[0, 1 - h], clean[0, 1 - h]), col
+
+
+@pytest.mark.parametrize("new", [1, 20, 64])
+def test_masses_under_another_lse(cuda, new):
+    """An lse that is not the row's own: the weights go by the formula, up to
+    infinity and down to 0."""
+    torch = cuda
+    c = P.make(torch, [new], [512], hq=8, hk=2)
+    _, lse = kv(c).attend(c["q"], *call(c), return_lse=True)
+    for off in (-50.0, 30.0):
+        mass = kv(c).block_mass(c["q"], lse + off, *call(c))
+        P.check_mass(c, mass, lse + off, 128 ** -0.5)
+    there = (512 + new + 15) // 16
+    mass = kv(c).block_mass(c["q"], lse - 200, *call(c))
+    assert (mass[:, :, :there] == math.inf).all() and (mass[:, :, there:] == 0).all()
+    mass = kv(c).block_mass(c["q"], lse + 200, *call(c))
+    assert (mass >= 0).all() and (mass < 1e-30).all()
+    # one row's lse too small, in every place of a tile of 128 rows
+    if new < 64:
+        return
+    for col in range(128):
+        row, h = col // 4, col % 4
+        l = lse.clone()
+        l[row, h] -= 200
+        mass = kv(c).block_mass(c["q"], l, *call(c))
+        seen = (512 + row) // 16 + 1
+        assert (mass[0, 0, :seen] == math.inf).all(), col
+        assert torch.isfinite(mass[0, 1]).all() and (mass >= 0).all(), col
