@@ -72,7 +72,8 @@ append_kernel(PagesDev p, BatchDev b, AppendDev a, uint32_t heads_per_warp, uint
             e1[u] = e0[u] + rest;
         }
     }
-    // of pair j of a unit; elements behind the rotated ones turn by nothing
+    // of pair j of a unit; elements behind the rotated ones turn by nothing, and
+    // their partners, be they infinite, have no part in them (rests)
     auto cosine = [&](int u, int j) {
         const uint32_t pr = (u * GL + gl) * VEC + j;
         return pr < half ? cos_s[pr] : 1.f;
@@ -81,6 +82,8 @@ append_kernel(PagesDev p, BatchDev b, AppendDev a, uint32_t heads_per_warp, uint
         const uint32_t pr = (u * GL + gl) * VEC + j;
         return pr < half ? sin_s[pr] : 0.f;
     };
+    const bool some_rest = rot < D;
+    auto rests = [&](int u, int j) { return some_rest && (u * GL + gl) * VEC + j >= half; };
 
     const uint32_t H = p.H, slots = a.Hq + 2 * H;
     const uint32_t first = ch * heads_per_warp, last = min(first + heads_per_warp, slots);
@@ -183,12 +186,14 @@ append_kernel(PagesDev p, BatchDev b, AppendDev a, uint32_t heads_per_warp, uint
                     const float *xa = x[k][0][u], *xb = x[k][1][u];
 #pragma unroll
                     for (int j = 0; j < VEC; j++) {
+                        y0[j] = xa[j] * f[0][u][j];
+                        y1[j] = xb[j] * f[2][u][j];
                         if (INTER && VEC > 1) {
-                            y0[j] = xa[j] * f[0][u][j] + xa[j ^ 1] * f[1][u][j];
-                            y1[j] = xb[j] * f[2][u][j] + xb[j ^ 1] * f[3][u][j];
-                        } else {
-                            y0[j] = xa[j] * f[0][u][j] + xb[j] * f[1][u][j];
-                            y1[j] = xb[j] * f[2][u][j] + xa[j] * f[3][u][j];
+                            if (!rests(u, j / 2)) y0[j] += xa[j ^ 1] * f[1][u][j];
+                            if (!rests(u, VEC / 2 + j / 2)) y1[j] += xb[j ^ 1] * f[3][u][j];
+                        } else if (!rests(u, 0)) {     // a vector's pairs all turn or all rest
+                            y0[j] += xb[j] * f[1][u][j];
+                            y1[j] += xa[j] * f[3][u][j];
                         }
                         if (nw) {
                             y0[j] *= inv;

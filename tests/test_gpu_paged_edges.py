@@ -151,3 +151,41 @@ def test_masses_under_another_lse(cuda, new):
         seen = (512 + row) // 16 + 1
         assert (mass[0, 0, :seen] == math.inf).all(), col
         assert torch.isfinite(mass[0, 1]).all() and (mass >= 0).all(), col
+
+
+# ---- append: elements that do not turn -------------------------------------------------
+
+@pytest.mark.parametrize("d,rot,inter", [(128, 0, False), (64, 32, False), (128, 64, True), (72, 20, False),
+                                         (256, 2, True), (40, 6, True), (128, 112, False), (64, 64, False)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("normed", [False, True])
+def test_append_elements_that_do_not_turn(cuda, d, rot, inter, dtype, normed):
+    """An infinite or NaN element that is not rotated stays where it is and
+    reaches no other; without a norm, such elements keep their very bits."""
+    torch = cuda
+    from orchkv_b200 import paged
+    c = P.make(torch, [9, 20], [0, 30], hq=6, hk=3, d=d, dtype=dtype, stale=3.0, seed=d + rot)
+    tail = torch.arange(rot, d, device="cuda")
+    for x in (c["q"], c["k"]):
+        for r in range(x.shape[0]):
+            for h in range(x.shape[1]):
+                if len(tail):
+                    at = tail[(7 * r + 3 * h) % len(tail)]
+                    x[r, h, at] = (math.inf, -math.inf, math.nan, -0.0)[(r + h) % 4]
+    w = torch.rand(d, generator=c["gen"], device="cuda").add(0.5).to(c["dt"]) if normed else None
+    freq = 10000.0 ** (-torch.arange(0, rot, 2, dtype=torch.float64, device="cuda") / max(rot, 1)) if rot else None
+    ro = paged.Rotary(d, inv_freq=freq, interleaved=inter, scale=1.25) if rot else None
+    want = M.append(c["kp"], c["vp"], c["layout"], *call(c), c["k"], c["v"], c["q"], freq, inter, 1.25, None, w, w)
+    got = kv(c).append(c["k"], c["v"], *call(c), q=c["q"], rotary=ro, q_norm=w, k_norm=w)
+    u = P.half_step(c["dt"])
+    for a, b in ((got, want[2]), (c["kp"], want[0])):
+        fin = torch.isfinite(b)
+        assert torch.equal(torch.isnan(a), torch.isnan(b))
+        assert torch.equal(a[torch.isinf(b)].double(), b[torch.isinf(b)])
+        amax = torch.where(fin, b, torch.zeros_like(b)).abs().amax(-1, keepdim=True)
+        tol = u * 1.01 * b.abs() + (d + 16) * 2.0 ** -24 * 1.25 * math.sqrt(2) * amax + 2.0 ** -25
+        assert ((a.double() - b).abs() <= tol)[fin].all()
+    if not normed:
+        same, x = got[..., rot:], c["q"][..., rot:]
+        ok = ~torch.isnan(x)
+        assert torch.equal(same[ok], x[ok]) and torch.equal(torch.signbit(same[ok]), torch.signbit(x[ok]))
