@@ -439,10 +439,11 @@ mass_runs_kernel(Geo g, PagesDev p, BatchDev b, MassDev a, uint32_t run, uint32_
 
         uint32_t qf[DP / 16][4];
         load_q_frag<T, DP>(a.q, r0, r1, D, qf);
-        // a row behind the last weighs nothing
+        // a row behind the last weighs nothing, whatever its zeros make of a key
+        const bool on0 = r0.row >= 0, on1 = r1.row >= 0;
         float ls[2];
-        ls[0] = r0.row >= 0 ? a.lse[(size_t)r0.row * a.Hq + r0.head] * kLog2e : INFINITY;
-        ls[1] = r1.row >= 0 ? a.lse[(size_t)r1.row * a.Hq + r1.head] * kLog2e : INFINITY;
+        ls[0] = on0 ? a.lse[(size_t)r0.row * a.Hq + r0.head] * kLog2e : 0.f;
+        ls[1] = on1 ? a.lse[(size_t)r1.row * a.Hq + r1.head] * kLog2e : 0.f;
 
         // the next group to load (block, group in it) and to weigh; a lane
         // holds the pages of two blocks of the run (of at most 64)
@@ -493,7 +494,9 @@ mass_runs_kernel(Geo g, PagesDev p, BatchDev b, MassDev a, uint32_t run, uint32_
                     float e[8];
 #pragma unroll
                     for (int j = 0; j < 8; j++) e[j] = ex2(sc[j >> 2][j & 3] * a.sl2 - ls[j >> 1 & 1]);
-                    part += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+                    const float w0 = on0 ? e[0] + e[1] : 0.f, w1 = on1 ? e[2] + e[3] : 0.f;
+                    const float w2 = on0 ? e[4] + e[5] : 0.f, w3 = on1 ? e[6] + e[7] : 0.f;
+                    part += (w0 + w1) + (w2 + w3);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; j++) {

@@ -1006,7 +1006,9 @@ mass_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                         if (lane == 0) mbar_arrive(smem_addr(&sh.s_empty[sb]));
                     }
                     const float4 *ls = (const float4 *)&sh.lse[st][c * 32];
-                    if (all) {
+                    // (columns of no row are masked: their zeros times an
+                    // infinite key are not 0)
+                    if (all && cols >= c * 32 + 32) {
 #pragma unroll
                         for (int j = 0; j < 8; j++) {
                             const float4 l4 = ls[j];

@@ -189,3 +189,28 @@ def test_append_elements_that_do_not_turn(cuda, d, rot, inter, dtype, normed):
         same, x = got[..., rot:], c["q"][..., rot:]
         ok = ~torch.isnan(x)
         assert torch.equal(same[ok], x[ok]) and torch.equal(torch.signbit(same[ok]), torch.signbit(x[ok]))
+
+
+@pytest.mark.parametrize("hq,hk", [(7, 1), (28, 4), (40, 1), (4, 4), (16, 1)])
+@pytest.mark.parametrize("new,block", [(1, 16), (1, 7), (5, 16), (70, 16), (300, 64)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_keys_of_no_weight(cuda, hq, hk, new, block, dtype):
+    """Keys whose score is minus infinity for every row weigh nothing, also
+    where a tile has places that hold no row."""
+    torch = cuda
+    d = 64
+    c = P.make(torch, [new], [500], hq=hq, hk=hk, d=d, block=block, dtype=dtype)
+    c["q"][:, :, 0] = c["q"][:, :, 0].abs() + 0.125
+    tok = torch.tensor([0, 3, 100, 101, 255, 256, 499], device="cuda")
+    c["kp"][c["table"][0, tok // block].long(), tok % block, :, 0] = -math.inf
+    out, lse = kv(c).attend(c["q"], *call(c), return_lse=True)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    mass = kv(c).block_mass(c["q"], lse, *call(c))
+    want = M.block_mass(c["kp"], c["layout"], *call(c), c["q"], lse, d ** -0.5)
+    # the bound of check_mass, its largest score taken over the other keys
+    kp = c["kp"].clone()
+    kp[torch.isinf(kp)] = 0
+    _, _, _, top = M.attend(kp, kp, c["layout"], *call(c), c["q"], d ** -0.5)
+    big = float(lse.abs().max())
+    rel = float(P.score_slack(torch.tensor(float(top.max()) + 2 * big / (d + 4), dtype=torch.float64), d)) + 2.0 ** -18
+    assert ((mass.double() - want).abs() <= rel * want + 1e-30).all()
