@@ -7,7 +7,7 @@
 // stream are taken care of here.  Arguments that do not fit raise ValueError,
 // a failed call RuntimeError.
 #include <ATen/ATen.h>
-#include <c10/core/GradMode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
@@ -41,8 +41,9 @@ class Pages {
 public:
     // heads 0: pages of one head each, as many heads as a call's table has
     Pages(int device, uintptr_t k, uintptr_t v, int64_t page, int64_t head, int64_t token, uint32_t n_pages,
-          uint32_t page_tokens, uint32_t heads, uint32_t d_head, int dtype)
-        : dev_(device), slab_(heads == 0), type_(scalar_of(dtype)),
+          uint32_t page_tokens, uint32_t heads, uint32_t d_head, int dtype, OptTensor k_pages, OptTensor v_pages)
+        : dev_(device), slab_(heads == 0), type_(scalar_of(dtype)), k_pages_(std::move(k_pages)),
+          v_pages_(std::move(v_pages)),
           pg_{reinterpret_cast<void *>(k), reinterpret_cast<void *>(v), page, head, token, n_pages, page_tokens,
               heads, d_head, dtype}
     {
@@ -54,6 +55,7 @@ public:
                       const OptTensor &k_norm, double eps, OptTensor q_out) const
     {
         const int64_t rows = k.dim() == 3 ? k.size(0) : -1;
+        no_gradient_of_pages();
         orchkv_batch_t b;
         const orchkv_pages_t pg = batch(table, lens, starts, rows, std::nullopt, &b);
         orchkv_append_args_t a = {};
@@ -84,11 +86,15 @@ public:
             if (turns->scalar_type() != at::kDouble || turns->dim() != 1 || !turns->is_contiguous() ||
                 !here(*turns) || 2 * turns->size(0) > (int64_t)pg.d_head)
                 refuse("rotary wider than a head, or on another device");
+            no_gradient(*turns, "rotary");
             a.turns = turns->data_ptr<double>();
             a.rot_dim = 2 * (uint32_t)turns->size(0);
         }
         c10::cuda::CUDAGuard guard(dev_);
         run(orchkv_paged_append(&pg, &b, &a, stream()), "paged_append");
+        if (k_pages_) written(*k_pages_);
+        if (v_pages_) written(*v_pages_);
+        if (q_out) written(*q_out);
         return q_out ? py::cast(*q_out) : py::none();
     }
 
@@ -98,6 +104,7 @@ public:
     {
         orchkv_batch_t b;
         orchkv_attend_args_t a = {};
+        no_gradient_of_pages();
         a.q = row_tensor(q, "q", -1, -1);
         const int64_t rows = q.size(0), hq = q.size(1);
         const orchkv_pages_t pg = batch(table, lens, starts, rows, max_new, &b);
@@ -115,6 +122,7 @@ public:
         Tensor ws;
         if (need) ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
         run(orchkv_paged_attend(&pg, &b, &a, need ? ws.data_ptr() : nullptr, need, stream()), "paged_attend");
+        written(*out);
         if (return_lse) return py::make_tuple(*out, lse);
         return py::cast(*out);
     }
@@ -125,6 +133,7 @@ public:
     {
         orchkv_batch_t b;
         orchkv_mass_args_t a = {};
+        no_gradient_of_pages();
         a.q = row_tensor(q, "q", -1, -1);
         const int64_t rows = q.size(0), hq = q.size(1);
         const orchkv_pages_t pg = batch(table, lens, starts, rows, max_new, &b);
@@ -132,6 +141,7 @@ public:
         if (lse.scalar_type() != at::kFloat || lse.dim() != 2 || lse.size(0) != rows || lse.size(1) != hq ||
             !lse.is_contiguous() || !here(lse))
             refuse("lse must be fp32 [rows, query heads], contiguous, on the pages' device");
+        no_gradient(lse, "lse");
         a.lse = lse.data_ptr<float>();
         c10::cuda::CUDAGuard guard(dev_);
         const int64_t shape[3] = {b.n_seqs, pg.n_kv_heads, b.table_width};
@@ -141,17 +151,37 @@ public:
                    !out->is_contiguous() || !here(*out)) {
             refuse("out must be fp32 [sequences, KV heads, table width], contiguous, on the pages' device");
         }
+        no_gradient(*out, "out");
         a.mass = out->data_ptr<float>();
         const size_t need = orchkv_paged_block_mass_workspace(&pg, &b, &a);
         Tensor ws;
         if (need) ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
         run(orchkv_paged_block_mass(&pg, &b, &a, need ? ws.data_ptr() : nullptr, need, stream()),
             "paged_block_mass");
+        written(*out);
         return py::cast(*out);
     }
 
 private:
     bool here(const Tensor &t) const { return t.is_cuda() && t.get_device() == dev_; }
+    // Every tensor a result depends on: a gradient, backward or forward, would be
+    // dropped here.
+    static void no_gradient(const Tensor &x, const char *name)
+    {
+        const c10::AutogradState &on = c10::AutogradState::get_tls_state();
+        if ((on.get_grad_mode() && x.requires_grad()) || (on.get_fw_grad_mode() && x._fw_grad(0).defined()))
+            refuse(std::string(name) + " requires a gradient, which these operators do not have");
+    }
+    void no_gradient_of_pages() const
+    {
+        if (k_pages_) no_gradient(*k_pages_, "k pages");
+        if (v_pages_) no_gradient(*v_pages_, "v pages");
+    }
+    // A tensor that a backward pass has saved is known to have changed.
+    static void written(const Tensor &x)
+    {
+        if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+    }
     void *stream() const { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev_).stream(); }
 
     // The pages as this call's tables see them, and its sequences.
@@ -198,8 +228,7 @@ private:
                           reinterpret_cast<uintptr_t>(x.data_ptr()) % 16))
             refuse(std::string(name) + ": heads must be contiguous, pointer and strides multiples of 16 bytes");
         if (!here(x)) refuse(std::string(name) + " must be on the pages' device");
-        if (x.requires_grad() && c10::GradMode::is_enabled())
-            refuse(std::string(name) + " requires a gradient, which these operators do not have");
+        no_gradient(x, name);
         return orchkv_rows_t{x.data_ptr(), x.stride(0), x.stride(1)};
     }
 
@@ -210,6 +239,7 @@ private:
             !w->is_contiguous() || !here(*w))
             refuse(std::string(name) + " must be [" + std::to_string(pg_.d_head) +
                    "] of the pages' dtype, contiguous, on the pages' device");
+        no_gradient(*w, name);
         return w->data_ptr();
     }
 
@@ -228,6 +258,7 @@ private:
     int dev_;
     bool slab_;
     at::ScalarType type_;
+    OptTensor k_pages_, v_pages_;          // none: memory that is no tensor
     orchkv_pages_t pg_;
 };
 
@@ -238,10 +269,10 @@ PYBIND11_MODULE(orchkv_torch, m)
     m.doc() = "OrchKvCache (B200): operators over paged caches on torch tensors";
     py::class_<Pages>(m, "Pages")
         .def(py::init<int, uintptr_t, uintptr_t, int64_t, int64_t, int64_t, uint32_t, uint32_t, uint32_t, uint32_t,
-                      int>(),
+                      int, OptTensor, OptTensor>(),
              py::arg("device"), py::arg("k_ptr"), py::arg("v_ptr"), py::arg("page_stride"), py::arg("head_stride"),
              py::arg("token_stride"), py::arg("n_pages"), py::arg("page_tokens"), py::arg("heads"),
-             py::arg("d_head"), py::arg("dtype"))
+             py::arg("d_head"), py::arg("dtype"), py::arg("k_pages"), py::arg("v_pages"))
         .def("append", &Pages::append)
         .def("attend", &Pages::attend)
         .def("block_mass", &Pages::block_mass);

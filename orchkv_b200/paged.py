@@ -22,7 +22,10 @@ attended over what is there.  Lengths and tables are read on the device: a
 captured call follows them.
 
 Everything runs on torch's current stream of the cache's device and keeps no
-state between calls.  The operators have no gradient.
+state between calls.  The operators have no gradient: an input that requires
+one (a norm's weight, frequencies, lse and the pages among them) is refused
+unless gradients are off, and tensors that a call writes into count as changed
+in place.
 """
 from __future__ import annotations
 
@@ -173,7 +176,7 @@ class PagedKV:
         self.n_pages, self.page_tokens, self.head_dim, self.dtype = n_pages, tokens, head_dim, dtype
         self.n_kv_heads = heads                   # None: as many as the call's tables have
         self._ops = torch_ops().Pages(device, k_ptr, v_ptr, *strides, n_pages, tokens, heads or 0,
-                                      head_dim, _DTYPES[dtype])
+                                      head_dim, _DTYPES[dtype], self.k, self.v)
 
     @classmethod
     def over_pool(cls) -> "PagedKV":

@@ -214,3 +214,84 @@ def test_keys_of_no_weight(cuda, hq, hk, new, block, dtype):
     big = float(lse.abs().max())
     rel = float(P.score_slack(torch.tensor(float(top.max()) + 2 * big / (d + 4), dtype=torch.float64), d)) + 2.0 ** -18
     assert ((mass.double() - want).abs() <= rel * want + 1e-30).all()
+
+
+# ---- gradients ----------------------------------------------------------------------------
+
+def test_gradients_are_refused_and_never_dropped(cuda):
+    torch = cuda
+    from orchkv_b200 import paged
+    c = P.make(torch, [2, 1], [5, 30], hq=4, hk=2)
+    x, a, d = kv(c), call(c), 128
+    w = torch.ones(d, dtype=c["dt"], device="cuda")
+    leaf = w.clone().requires_grad_()
+    freq = torch.ones(d // 2, device="cuda").requires_grad_()
+    lse = torch.zeros(3, 4, device="cuda")
+    grad_lse = lse.clone().requires_grad_()
+    learned = paged.Rotary(d, inv_freq=freq)
+    hot = paged.PagedKV(c["kp"].float().requires_grad_().to(c["dt"]), c["vp"])
+    calls = [
+        lambda **k: x.append(c["k"], c["v"], *a, q=c["q"], q_norm=leaf),
+        lambda **k: x.append(c["k"], c["v"], *a, k_norm=leaf),
+        lambda **k: x.append(c["k"], c["v"], *a, rotary=learned),
+        lambda **k: x.block_mass(c["q"], grad_lse, *a),
+        lambda **k: hot.append(c["k"], c["v"], *a),
+        lambda **k: hot.attend(c["q"], *a),
+        lambda **k: hot.block_mass(c["q"], lse, *a),
+    ]
+    for i, fn in enumerate(calls):
+        with pytest.raises(ValueError, match="gradient"):
+            fn()
+        with torch.no_grad():
+            fn()
+
+
+def test_forward_gradients_are_refused(cuda):
+    torch = cuda
+    import torch.autograd.forward_ad as fwd
+    c = P.make(torch, [2, 1], [5, 30], hq=4, hk=2)
+    x, a = kv(c), call(c)
+    w = torch.ones(128, dtype=c["dt"], device="cuda")
+    lse = torch.zeros(3, 4, device="cuda")
+    with fwd.dual_level():
+        def dual(t):
+            return fwd.make_dual(t, torch.ones_like(t))
+        for fn in (lambda: x.attend(dual(c["q"]), *a), lambda: x.append(dual(c["k"]), c["v"], *a),
+                   lambda: x.append(c["k"], c["v"], *a, k_norm=dual(w)),
+                   lambda: x.block_mass(c["q"], dual(lse), *a)):
+            with pytest.raises(ValueError, match="gradient"):
+                fn()
+
+
+def test_a_tensor_saved_for_a_backward_pass_and_overwritten_is_noticed(cuda):
+    torch = cuda
+    c = P.make(torch, [2, 1], [5, 30], hq=4, hk=2, dtype="fp32")
+    x, a = kv(c), call(c)
+    leaf = torch.ones((), device="cuda", requires_grad=True)
+    lse = torch.zeros(3, 4, device="cuda")
+
+    def written(t, fn):
+        """fn writes into t, which the product has saved."""
+        y = (leaf * t).sum()
+        fn()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+
+    q = c["q"].clone()
+    written(q, lambda: x.append(c["k"], c["v"], *a, q=q, q_out=q))
+    written(c["kp"], lambda: x.append(c["k"], c["v"], *a))
+    written(c["vp"], lambda: x.append(c["k"], c["v"], *a))
+    out = torch.empty_like(c["q"])
+    written(out, lambda: x.attend(c["q"], *a, out=out))
+    mass = torch.empty(2, 2, c["table"].shape[1], device="cuda")
+    written(mass, lambda: x.block_mass(c["q"], lse, *a, out=mass))
+
+
+def test_inference_tensors(cuda):
+    torch = cuda
+    with torch.inference_mode():
+        c = P.make(torch, [2, 1], [5, 30], hq=4, hk=2)
+        q = kv(c).append(c["k"], c["v"], *call(c), q=c["q"], q_out=c["q"])
+        out, lse = kv(c).attend(q, *call(c), return_lse=True, out=torch.empty_like(q))
+    P.check_attend(c, out, lse, 128 ** -0.5)
+    kv(c).append(c["k"], c["v"], *call(c), q=c["q"], q_out=c["q"])   # and outside of it
