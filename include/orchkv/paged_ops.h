@@ -89,7 +89,8 @@ typedef struct orchkv_append_args {
 
 /* x of a q or k head: y = x / sqrt(mean(x^2) + eps) * norm, if a norm is
  * given; y rotated, in fp32 and rounded once; k and v into the pages, q to
- * q_out (which may be q).  Tokens whose table entry names no page are not
+ * q_out (which may be q itself; else it must not overlap q, and never k, v or
+ * itself).  Tokens whose table entry names no page are not
  * written (their q still is).  Asynchronous. */
 int orchkv_paged_append(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
                         const orchkv_append_args_t *args, void *stream);
@@ -109,7 +110,7 @@ typedef struct orchkv_attend_args {
  * What lies in places that a row does not attend to does not reach it, be it
  * infinite or NaN; an infinite or NaN value reaches every row that does, as
  * such or as NaN.
- * out must not overlap q.
+ * out must not overlap q or itself.
  * workspace: orchkv_paged_attend_workspace() bytes of device memory, 256-byte
  * aligned, of this call alone until it has run.  Asynchronous. */
 size_t orchkv_paged_attend_workspace(const orchkv_pages_t *pages, const orchkv_batch_t *batch,

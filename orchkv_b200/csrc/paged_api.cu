@@ -4,6 +4,7 @@
 
 #include "kernels.h"
 #include "paged.cuh"
+#include "paged_overlap.h"
 
 using namespace okv;
 
@@ -180,6 +181,16 @@ int orchkv_paged_append(const orchkv_pages_t *pages, const orchkv_batch_t *batch
     if (batch->n_rows == 0 || batch->n_seqs == 0) return ORCHKV_OK;
     if (!rows_ok(args->k, e) || !rows_ok(args->v, e)) return ORCHKV_ERR_INVALID;
     if (args->n_q_heads && (!rows_ok(args->q, e) || !rows_ok(args->q_out, e))) return ORCHKV_ERR_INVALID;
+    const auto span = [&](const orchkv_rows_t &r, uint32_t heads) {
+        return row_span(r, batch->n_rows, heads, (int64_t)(pages->d_head * e), (int64_t)e);
+    };
+    if (args->n_q_heads) {
+        // (other CTAs read what one of them writes)
+        const RowSpan q = span(args->q, args->n_q_heads), o = span(args->q_out, args->n_q_heads);
+        if (overlaps_itself(o) || (!same_rows(q, o) && overlap(q, o)) ||
+            overlap(o, span(args->k, pages->n_kv_heads)) || overlap(o, span(args->v, pages->n_kv_heads)))
+            return ORCHKV_ERR_INVALID;
+    }
     if (args->n_q_heads > 65535 ||
         (uint64_t)batch->n_rows * (args->n_q_heads + 2ull * pages->n_kv_heads) > 0x7FFFFFFFull)
         return ORCHKV_ERR_INVALID;
@@ -218,8 +229,11 @@ int orchkv_paged_attend(const orchkv_pages_t *pages, const orchkv_batch_t *batch
         return ORCHKV_ERR_INVALID;
     if (batch->n_rows == 0 || batch->n_seqs == 0) return ORCHKV_OK;
     const size_t e = dtype_size((DataType)pages->dtype);
+    if (!rows_ok(args->q, e) || !rows_ok(args->out, e)) return ORCHKV_ERR_INVALID;
     // (several CTAs read a row of q that one of them writes the result of)
-    if (!rows_ok(args->q, e) || !rows_ok(args->out, e) || args->q.p == args->out.p) return ORCHKV_ERR_INVALID;
+    const RowSpan qs = row_span(args->q, batch->n_rows, args->n_q_heads, (int64_t)(pages->d_head * e), (int64_t)e);
+    const RowSpan os = row_span(args->out, batch->n_rows, args->n_q_heads, (int64_t)(pages->d_head * e), (int64_t)e);
+    if (overlap(qs, os) || overlaps_itself(os)) return ORCHKV_ERR_INVALID;
     AttendPlan pl = plan_attend(pages, batch, args);
     if (pl.bytes && (!workspace || (uintptr_t)workspace % 256 || bytes < pl.bytes)) return ORCHKV_ERR_INVALID;
     AttendDev a;

@@ -17,6 +17,7 @@
 #include <string>
 
 #include "orchkv/paged_ops.h"
+#include "paged_overlap.h"
 
 namespace py = pybind11;
 using at::Tensor;
@@ -66,6 +67,11 @@ public:
             a.n_q_heads = (uint32_t)q->size(1);
             if (!q_out) q_out = at::empty(q->sizes(), q->options());
             a.q_out = row_tensor(*q_out, "q_out", a.n_q_heads, rows);
+            const okv::RowSpan qs = span(a.q, a.n_q_heads, rows), os = span(a.q_out, a.n_q_heads, rows);
+            if (!okv::same_rows(qs, os) && okv::overlap(qs, os)) refuse("q_out must be q itself or not overlap it");
+            if (okv::overlaps_itself(os)) refuse("q_out: rows and heads must not overlap");
+            if (okv::overlap(os, span(a.k, pg.n_kv_heads, rows)) || okv::overlap(os, span(a.v, pg.n_kv_heads, rows)))
+                refuse("q_out must not overlap k and v");
         } else if (q_out || q_norm) {
             refuse("q_out and q_norm go with q");
         }
@@ -112,7 +118,8 @@ public:
         c10::cuda::CUDAGuard guard(dev_);
         if (!out) out = at::empty(q.sizes(), q.options());
         a.out = row_tensor(*out, "out", hq, rows);
-        if (rows && a.out.p == a.q.p) refuse("out must not overlap q");
+        if (okv::overlap(span(a.q, hq, rows), span(a.out, hq, rows))) refuse("out must not overlap q");
+        if (okv::overlaps_itself(span(a.out, hq, rows))) refuse("out: rows and heads must not overlap");
         Tensor lse;
         if (return_lse) {
             lse = at::empty({rows, hq}, q.options().dtype(at::kFloat));
@@ -230,6 +237,12 @@ private:
         if (!here(x)) refuse(std::string(name) + " must be on the pages' device");
         no_gradient(x, name);
         return orchkv_rows_t{x.data_ptr(), x.stride(0), x.stride(1)};
+    }
+
+    okv::RowSpan span(const orchkv_rows_t &r, int64_t heads, int64_t rows) const
+    {
+        const int64_t e = type_ == at::kFloat ? 4 : 2;
+        return okv::row_span(r, rows, heads, pg_.d_head * e, e);
     }
 
     const void *norm(const OptTensor &w, const char *name) const

@@ -295,3 +295,62 @@ def test_inference_tensors(cuda):
         out, lse = kv(c).attend(q, *call(c), return_lse=True, out=torch.empty_like(q))
     P.check_attend(c, out, lse, 128 ** -0.5)
     kv(c).append(c["k"], c["v"], *call(c), q=c["q"], q_out=c["q"])   # and outside of it
+
+
+# ---- tensors that share memory ---------------------------------------------------------
+
+def test_overlapping_tensors_are_refused(cuda):
+    torch = cuda
+    c = P.make(torch, [3, 1], [5, 30], hq=4, hk=2)
+    x, a, d = kv(c), call(c), 128
+    buf = torch.zeros(40, d, dtype=c["dt"], device="cuda")
+    q = buf[:16].view(4, 4, d)
+    later, one = buf[4:20].view(4, 4, d), buf[:4].view(1, 4, d).expand(4, 4, d)
+    flat = buf[:4].view(4, 1, d).expand(4, 4, d)
+    for out in (later, buf[15:31].view(4, 4, d), q):
+        with pytest.raises(ValueError, match="overlap"):
+            x.attend(q, *a, out=out)
+    for out in (later, one, flat):
+        with pytest.raises(ValueError, match="overlap"):
+            x.append(c["k"], c["v"], *a, q=q, q_out=out)
+    for out in (one, flat):
+        with pytest.raises(ValueError, match="overlap"):
+            x.attend(c["q"], *a, out=out)
+    k = buf[8:16].view(4, 2, d)
+    with pytest.raises(ValueError, match="k and v"):
+        x.append(k, c["v"], *a, q=c["q"], q_out=buf[:16].view(4, 4, d))
+    with pytest.raises(ValueError, match="k and v"):
+        x.append(c["k"], k, *a, q=c["q"], q_out=buf[:16].view(4, 4, d))
+    # a broadcast input is an ordinary one
+    P.check_attend(dict(c, q=one), *x.attend(one, *a, return_lse=True), d ** -0.5)
+
+
+@pytest.mark.parametrize("how", ["rows", "heads", "columns", "in place"])
+def test_interleaved_tensors_are_taken(cuda, how):
+    """q and the results in one buffer, but in places of their own."""
+    torch = cuda
+    from orchkv_b200 import paged
+    c = P.make(torch, [3, 40], [5, 30], hq=4, hk=2)
+    T, d = 43, 128
+    if how == "rows":
+        buf = torch.zeros(2 * T, 4, d, dtype=c["dt"], device="cuda")
+        q, out = buf[0::2], buf[1::2]
+    elif how == "heads":
+        buf = torch.zeros(T, 4, 2, d, dtype=c["dt"], device="cuda")
+        q, out = buf[:, :, 0], buf[:, :, 1]
+    else:
+        buf = torch.zeros(T, 12, d, dtype=c["dt"], device="cuda")
+        q, out = buf[:, :4], buf[:, 4:8]
+        if how == "in place":
+            c["k"], c["v"] = buf[:, 8:10].copy_(c["k"]), buf[:, 10:].copy_(c["v"])
+    q.copy_(c["q"])
+    ro = paged.Rotary(d)
+    want = kv(c).append(c["k"], c["v"], *call(c), q=c["q"], rotary=ro)
+    if how == "in place":
+        assert kv(c).append(c["k"], c["v"], *call(c), q=q, rotary=ro, q_out=q) is q
+        assert torch.equal(q, want)
+    else:
+        assert kv(c).append(c["k"], c["v"], *call(c), q=q, rotary=ro, q_out=out) is out
+        assert torch.equal(out, want) and torch.equal(q, c["q"])
+    got = kv(c).attend(q, *call(c), out=out)
+    assert torch.equal(got, kv(c).attend(q.contiguous(), *call(c)))
