@@ -66,7 +66,10 @@ struct TileShared {
     ull full[8], empty[8], s_full[2], p_full[2], q_full[2], o_full[2], s_free, fix, drain;
     uint32_t tmem;
     int dead;
-    int odd[kMeta];                        // of a unit: values that are not finite behind some row's mask
+    // the last unit (counted from 1) of every kMeta with values that are not
+    // finite behind some row's mask; never reset, since a half may look at a
+    // unit long after the loads have left it
+    uint32_t odd[kMeta];
     alignas(16) uint32_t mask[kMeta][4];   // columns of a tile that hold a token
     SplitShared split;
 };
@@ -105,6 +108,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         mbar_init(smem_addr(&sh.s_free), 4);
         mbar_init(smem_addr(&sh.fix), 1);
         mbar_init(smem_addr(&sh.drain), 1);
+        for (int k = 0; k < kMeta; k++) sh.odd[k] = 0;
         sh.dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -138,7 +142,6 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             // keys that every row of the unit attends to
             const int all_hi = row_info(g, w.s, h, w.at.rt * kR).hi;
             const int all_lo = row_info(g, w.s, h, w.at.rt * kR + w.live() - 1).lo;
-            if (is_v && lane == 0) sh.odd[u_no % kMeta] = 0;
             auto page = [&](uint32_t t) {                  // lane q: page q of tile t
                 if (t >= w.t1 || lane >= per) return -1;
                 const uint32_t k0 = (w.first + t) * kK + lane * bs;
@@ -225,7 +228,7 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                                 if (infinite<T>(v, 1)) v &= 0xFFFFu;
                                 asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + e * 4), "r"(v) : "memory");
                             }
-                            if (lane == 0) sh.odd[u_no % kMeta] = 1;
+                            if (lane == 0) sh.odd[u_no % kMeta] = u_no + 1;
                         }
                     }
                     fence_async();
@@ -492,7 +495,8 @@ attend_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             unf2(l2[0], &la, &lb);
             unf2(l2[1], &lc, &ld);
             const float L = (la + lb) + (lc + ld);
-            const bool whole = w.t0 == 0 && w.t1 == w.nt, odd = sh.odd[u_no % kMeta] != 0;
+            // (a later unit of the same place asks for a look that finds nothing)
+            const bool whole = w.t0 == 0 && w.t1 == w.nt, odd = sh.odd[u_no % kMeta] > u_no;
             const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
             float *sl = slot_of(sp.ws, 2 * blockIdx.x + (w.t0 == 0 ? 1 : 0), kR, p.D);
             char *dst = a.out.p + (long long)ri.row * a.out.row_b + (long long)ri.head * a.out.head_b;

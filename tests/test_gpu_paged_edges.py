@@ -354,3 +354,31 @@ def test_interleaved_tensors_are_taken(cuda, how):
         assert torch.equal(out, want) and torch.equal(q, c["q"])
     got = kv(c).attend(q, *call(c), out=out)
     assert torch.equal(got, kv(c).attend(q.contiguous(), *call(c)))
+
+
+# ---- units of one half behind a unit of two ------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_infinite_values_before_many_short_sequences(cuda, dtype, bad):
+    """Long sequences with a value that is not finite on their diagonal, each
+    before dozens of short ones that need half a tile only: the rows that
+    attend to it are not finite, all others are as without it."""
+    torch = cuda
+    new = ([300] + [40] * 60) * 6
+    held = [30] * len(new)
+    c = P.make(torch, new, held, hq=8, hk=8, dtype=dtype, seed=3)
+    want, wl = kv(c).attend(c["q"], *call(c), return_lse=True)
+    at = 30 + 200
+    for i in range(0, len(new), 61):
+        page = int(c["table"][i, at // 16])
+        c["vp"][page, at % 16, :, 5:8] = bad
+    for _ in range(5):
+        out, lse = kv(c).attend(c["q"], *call(c), return_lse=True)
+        assert torch.equal(lse, wl)
+        hit = torch.zeros_like(out, dtype=torch.bool)
+        for i in range(0, len(new), 61):
+            r = int(c["starts"][i])
+            hit[r + 200:r + 300, :, 5:8] = True
+        assert not torch.isfinite(out[hit]).any()
+        assert torch.equal(out[~hit], want[~hit])
