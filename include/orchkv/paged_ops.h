@@ -91,7 +91,8 @@ typedef struct orchkv_append_args {
  * given; y rotated, in fp32 and rounded once; k and v into the pages, q to
  * q_out (which may be q itself; else it must not overlap q, and never k, v or
  * itself).  Tokens whose table entry names no page are not
- * written (their q still is).  Asynchronous. */
+ * written (their q still is).  Every place of the pages must have memory of its
+ * own (no zero stride over several pages, tokens or heads).  Asynchronous. */
 int orchkv_paged_append(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
                         const orchkv_append_args_t *args, void *stream);
 
@@ -132,7 +133,7 @@ typedef struct orchkv_mass_args {
  * g and the tokens t of block b of exp(scale * q[r, h] . K[t] - lse[r, h]),
  * the probability orchkv_paged_attend gave t: what tm_report_attn_probs sums
  * out of a stored map.  Blocks that hold no attended token get 0.  Sums run
- * in one fixed order.  pages->v is not read.  workspace as for
+ * in one fixed order.  pages->v is not read; mass must not overlap q or lse.  workspace as for
  * orchkv_paged_attend (NULL where the size is 0).  Asynchronous. */
 size_t orchkv_paged_block_mass_workspace(const orchkv_pages_t *pages, const orchkv_batch_t *batch,
                                          const orchkv_mass_args_t *args);

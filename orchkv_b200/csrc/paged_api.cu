@@ -41,6 +41,14 @@ bool shapes_ok(const orchkv_pages_t *p, const orchkv_batch_t *b, bool need_v)
     return true;
 }
 
+// Whether the places that an append writes differ: no zero stride over several
+// pages, tokens or (in one page for all heads) heads.
+bool places_ok(const orchkv_pages_t *p, const orchkv_batch_t *b)
+{
+    return (p->page_stride || p->n_pages == 1) && (p->token_stride || p->page_tokens == 1) &&
+           (p->head_stride || b->table_head_stride || p->n_kv_heads == 1);
+}
+
 bool heads_ok(const orchkv_pages_t *p, const orchkv_batch_t *b, uint32_t hq)
 {
     return hq != 0 && hq % p->n_kv_heads == 0 && (uint64_t)hq * b->n_rows < 0x7FFFFFFFull;
@@ -179,7 +187,7 @@ int orchkv_paged_append(const orchkv_pages_t *pages, const orchkv_batch_t *batch
     if (args->rot_dim % 2 || args->rot_dim > pages->d_head) return ORCHKV_ERR_INVALID;
     if (args->rot_dim && !args->turns) return ORCHKV_ERR_INVALID;
     if (batch->n_rows == 0 || batch->n_seqs == 0) return ORCHKV_OK;
-    if (!rows_ok(args->k, e) || !rows_ok(args->v, e)) return ORCHKV_ERR_INVALID;
+    if (!rows_ok(args->k, e) || !rows_ok(args->v, e) || !places_ok(pages, batch)) return ORCHKV_ERR_INVALID;
     if (args->n_q_heads && (!rows_ok(args->q, e) || !rows_ok(args->q_out, e))) return ORCHKV_ERR_INVALID;
     const auto span = [&](const orchkv_rows_t &r, uint32_t heads) {
         return row_span(r, batch->n_rows, heads, (int64_t)(pages->d_head * e), (int64_t)e);
@@ -272,6 +280,11 @@ int orchkv_paged_block_mass(const orchkv_pages_t *pages, const orchkv_batch_t *b
     if (batch->n_seqs == 0) return ORCHKV_OK;
     const size_t e = dtype_size((DataType)pages->dtype);
     if (!args->mass || (batch->n_rows && (!rows_ok(args->q, e) || !args->lse))) return ORCHKV_ERR_INVALID;
+    if (batch->n_rows) {
+        const RowSpan q = row_span(args->q, batch->n_rows, args->n_q_heads, (int64_t)(pages->d_head * e), (int64_t)e);
+        if (mass_overlaps(args->mass, batch->n_seqs, pages->n_kv_heads, batch->table_width, q, args->lse))
+            return ORCHKV_ERR_INVALID;
+    }
     MassPlan pl = plan_mass(pages, batch, args);
     if (pl.bytes && (!workspace || (uintptr_t)workspace % 256 || bytes < pl.bytes)) return ORCHKV_ERR_INVALID;
     MassDev a;

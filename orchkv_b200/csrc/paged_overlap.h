@@ -63,4 +63,14 @@ inline bool same_rows(const RowSpan &a, const RowSpan &b)
     return a.p == b.p && a.row == b.row && a.head == b.head;
 }
 
+// Whether the masses, which are written while q and lse are read, lie between
+// the first and last byte of either (of q's rows and heads).
+inline bool mass_overlaps(const float *mass, int64_t seqs, int64_t kv_heads, int64_t width, const RowSpan &q,
+                          const float *lse)
+{
+    const int64_t p = (int64_t)(uintptr_t)mass, e = p + 4 * seqs * kv_heads * width;
+    const int64_t l = (int64_t)(uintptr_t)lse, le = l + 4 * q.rows * q.heads;
+    return q.rows && p < e && ((p < q.end() && q.p < e) || (p < le && l < e));
+}
+
 }  // namespace okv

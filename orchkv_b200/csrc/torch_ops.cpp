@@ -96,6 +96,9 @@ public:
             a.turns = turns->data_ptr<double>();
             a.rot_dim = 2 * (uint32_t)turns->size(0);
         }
+        if ((!pg.page_stride && pg.n_pages > 1) || (!pg.token_stride && pg.page_tokens > 1) ||
+            (!pg.head_stride && !b.table_head_stride && pg.n_kv_heads > 1))
+            refuse("pages to write into must not be broadcast over pages, tokens or heads");
         c10::cuda::CUDAGuard guard(dev_);
         run(orchkv_paged_append(&pg, &b, &a, stream()), "paged_append");
         if (k_pages_) written(*k_pages_);
@@ -160,6 +163,8 @@ public:
         }
         no_gradient(*out, "out");
         a.mass = out->data_ptr<float>();
+        if (okv::mass_overlaps(a.mass, shape[0], shape[1], shape[2], span(a.q, hq, rows), a.lse))
+            refuse("out must not overlap q or lse");
         const size_t need = orchkv_paged_block_mass_workspace(&pg, &b, &a);
         Tensor ws;
         if (need) ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));

@@ -382,3 +382,18 @@ def test_infinite_values_before_many_short_sequences(cuda, dtype, bad):
             hit[r + 200:r + 300, :, 5:8] = True
         assert not torch.isfinite(out[hit]).any()
         assert torch.equal(out[~hit], want[~hit])
+
+
+def test_broadcast_pages_are_read_and_not_written(cuda):
+    """K and V shared by all heads: attended over like any, refused for an
+    append, whose heads would write one place; masses over their inputs."""
+    torch = cuda
+    c = P.make(torch, [2, 40], [90, 30], hq=4, hk=1)
+    shared = dict(c, kp=c["kp"].expand(-1, -1, 4, -1), vp=c["vp"].expand(-1, -1, 4, -1))
+    out, lse = kv(shared).attend(c["q"], *call(c), return_lse=True)
+    P.check_attend(shared, out, lse, 128 ** -0.5)
+    k4 = c["k"].expand(-1, 4, -1).contiguous()
+    with pytest.raises(ValueError, match="broadcast"):
+        kv(shared).append(k4, k4, *call(c))
+    with pytest.raises(ValueError, match="overlap"):
+        kv(c).block_mass(c["q"], lse, *call(c), out=lse.flatten()[:2 * c["table"].shape[1]].view(2, 1, -1))

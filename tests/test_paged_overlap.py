@@ -82,3 +82,13 @@ def test_the_rule_is_the_bytes(tmp_path):
             assert over >= share and (not over or (min(ta) <= max(tb) and min(tb) <= max(ta)))
         seen.add((over, share, itself))
     assert {(0, 0, 0), (1, 1, 0), (1, 1, 1), (0, 0, 1)} <= seen
+
+
+@pytest.mark.parametrize("bad,op", [
+    # several places of the pages in one memory
+    (dict(page_stride=0), "append"), (dict(token_stride=0), "append"), (dict(head_stride=0), "append"),
+    # masses over q or lse (which `call` has at the same address)
+    (dict(out=A), "mass"), (dict(out=A + 5 * ROW), "mass"), (dict(out=A - 4 * 4096 * 4), "mass"),
+])
+def test_broadcast_pages_and_masses_over_inputs(bad, op):
+    assert call(**bad)[1][op]() == INVALID
