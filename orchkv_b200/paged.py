@@ -129,6 +129,11 @@ class Rotary:
         raise ValueError(f"unknown scaling type {kind!r}")
 
 
+def _pool_device() -> int:
+    """The device of the data plane's GPU pool, once it is initialised."""
+    return C.cast(lib().orchkv_gpu_tier(), C.POINTER(C.c_int))[0]         # its first field
+
+
 def _need(ok: bool, msg: str):
     if not ok:
         raise ValueError(msg)
@@ -193,8 +198,7 @@ class PagedKV:
         self = cls.__new__(cls)
         self.k = self.v = None
         self.layout = "slab"
-        device = C.cast(lib().orchkv_gpu_tier(), C.POINTER(C.c_int))[0]   # its first field
-        self._set(device, pg.k, pg.v,
+        self._set(_pool_device(), pg.k, pg.v,
                   (pg.page_stride, pg.head_stride, pg.token_stride), pg.n_pages, pg.page_tokens, None,
                   pg.d_head, dtype)
         return self
@@ -245,9 +249,9 @@ def pool_table(requests, layer: int, row_len: int, n_kv_heads: int) -> tuple[tor
     if rc != 0:
         raise RuntimeError(f"orchkv_pool_pages failed: {rc}")
     _need(n_kv_heads > 0 and row_len > 0 and len(requests) > 0, "requests, heads and row_len must not be 0")
-    table = torch.empty(len(requests), n_kv_heads, -(-row_len // pg.page_tokens), dtype=torch.int32,
-                        device="cuda")
-    lens = torch.empty(len(requests), dtype=torch.int32, device="cuda")
+    device = torch.device("cuda", _pool_device())
+    table = torch.empty(len(requests), n_kv_heads, -(-row_len // pg.page_tokens), dtype=torch.int32, device=device)
+    lens = torch.empty(len(requests), dtype=torch.int32, device=device)
     rc = cpp.slab_table(list(requests), layer, n_kv_heads, row_len, table.data_ptr(), lens.data_ptr())
     if rc != 0:
         raise RuntimeError(f"orchkv_slab_table failed: {rc}")
