@@ -87,7 +87,6 @@ append_kernel(PagesDev p, BatchDev b, AppendDev a, uint32_t heads_per_warp, uint
 
     const uint32_t H = p.H, slots = a.Hq + 2 * H;
     const uint32_t first = ch * heads_per_warp, last = min(first + heads_per_warp, slots);
-    constexpr int U = 1;                 // heads in flight a lane
     // one page for all heads, or one each
     const int pg_all = in_table && b.ts_head == 0 ? page_of(b, p.n_pages, i, 0, blk) : -1;
     auto place = [&](char *base, uint32_t h) -> char * {
@@ -153,60 +152,53 @@ append_kernel(PagesDev p, BatchDev b, AppendDev a, uint32_t heads_per_warp, uint
             }
         const RowsDev &rw = is_q ? a.q : a.k;
         const char *src0 = rw.p + (long long)r * rw.row_b;
-        for (uint32_t h0 = lo; h0 < hi; h0 += U * HPW) {
-            float x[U][2][NU][VEC];
+        for (uint32_t h0 = lo; h0 < hi; h0 += HPW) {
+            const uint32_t h = h0 + gh;
+            float x[2][NU][VEC];
+            load(h < hi ? src0 + (long long)h * rw.head_b : nullptr, x);
+            float inv = 1.f;
+            if (nw) {                              // the lanes of a head reduce together
+                float ss = 0.f;
 #pragma unroll
-            for (int k = 0; k < U; k++) {
-                const uint32_t h = h0 + k * HPW + gh;
-                load(h < hi ? src0 + (long long)h * rw.head_b : nullptr, x[k]);
+                for (int u = 0; u < NU; u++)
+#pragma unroll
+                    for (int j = 0; j < VEC; j++)
+                        ss += x[0][u][j] * x[0][u][j] + x[1][u][j] * x[1][u][j];
+#pragma unroll
+                for (int o = GL / 2; o; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+                inv = rsqrtf(ss / (float)D + a.eps);
             }
+            if (h >= hi) continue;
+            char *dst = is_q ? a.q_out.p + (long long)r * a.q_out.row_b + (long long)h * a.q_out.head_b
+                             : place(p.k, h);
+            if (!dst) continue;
 #pragma unroll
-            for (int k = 0; k < U; k++) {
-                const uint32_t h = h0 + k * HPW + gh;
-                float inv = 1.f;
-                if (nw) {                              // the lanes of a head reduce together
-                    float ss = 0.f;
+            for (int u = 0; u < NU; u++) {
+                if (u * GL + gl >= units) continue;
+                float y0[VEC], y1[VEC];
+                const float *xa = x[0][u], *xb = x[1][u];
 #pragma unroll
-                    for (int u = 0; u < NU; u++)
-#pragma unroll
-                        for (int j = 0; j < VEC; j++)
-                            ss += x[k][0][u][j] * x[k][0][u][j] + x[k][1][u][j] * x[k][1][u][j];
-#pragma unroll
-                    for (int o = GL / 2; o; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-                    inv = rsqrtf(ss / (float)D + a.eps);
+                for (int j = 0; j < VEC; j++) {
+                    y0[j] = xa[j] * f[0][u][j];
+                    y1[j] = xb[j] * f[2][u][j];
+                    if (INTER && VEC > 1) {
+                        if (!rests(u, j / 2)) y0[j] += xa[j ^ 1] * f[1][u][j];
+                        if (!rests(u, VEC / 2 + j / 2)) y1[j] += xb[j ^ 1] * f[3][u][j];
+                    } else if (!rests(u, 0)) {     // a vector's pairs all turn or all rest
+                        y0[j] += xb[j] * f[1][u][j];
+                        y1[j] += xa[j] * f[3][u][j];
+                    }
+                    if (nw) {
+                        y0[j] *= inv;
+                        y1[j] *= inv;
+                    }
                 }
-                if (h >= hi) continue;
-                char *dst = is_q ? a.q_out.p + (long long)r * a.q_out.row_b + (long long)h * a.q_out.head_b
-                                 : place(p.k, h);
-                if (!dst) continue;
-#pragma unroll
-                for (int u = 0; u < NU; u++) {
-                    if (u * GL + gl >= units) continue;
-                    float y0[VEC], y1[VEC];
-                    const float *xa = x[k][0][u], *xb = x[k][1][u];
-#pragma unroll
-                    for (int j = 0; j < VEC; j++) {
-                        y0[j] = xa[j] * f[0][u][j];
-                        y1[j] = xb[j] * f[2][u][j];
-                        if (INTER && VEC > 1) {
-                            if (!rests(u, j / 2)) y0[j] += xa[j ^ 1] * f[1][u][j];
-                            if (!rests(u, VEC / 2 + j / 2)) y1[j] += xb[j ^ 1] * f[3][u][j];
-                        } else if (!rests(u, 0)) {     // a vector's pairs all turn or all rest
-                            y0[j] += xb[j] * f[1][u][j];
-                            y1[j] += xa[j] * f[3][u][j];
-                        }
-                        if (nw) {
-                            y0[j] *= inv;
-                            y1[j] *= inv;
-                        }
-                    }
-                    if constexpr (VEC > 1) {
-                        *(uint4 *)(dst + (size_t)e0[u] * sizeof(T)) = Vec<T>::down(y0);
-                        *(uint4 *)(dst + (size_t)e1[u] * sizeof(T)) = Vec<T>::down(y1);
-                    } else {
-                        ((T *)dst)[e0[u]] = from_f<T>(y0[0]);
-                        ((T *)dst)[e1[u]] = from_f<T>(y1[0]);
-                    }
+                if constexpr (VEC > 1) {
+                    *(uint4 *)(dst + (size_t)e0[u] * sizeof(T)) = Vec<T>::down(y0);
+                    *(uint4 *)(dst + (size_t)e1[u] * sizeof(T)) = Vec<T>::down(y1);
+                } else {
+                    ((T *)dst)[e0[u]] = from_f<T>(y0[0]);
+                    ((T *)dst)[e1[u]] = from_f<T>(y1[0]);
                 }
             }
         }

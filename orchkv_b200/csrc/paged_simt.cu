@@ -20,27 +20,21 @@ constexpr int R = kSimtRows;
 constexpr int kD = 256;
 
 // Scores of this lane's key against the R rows in q_s (already scaled).
-template <class T>
 __device__ __forceinline__ void dots(const char *krow, const float (*q_s)[kD], uint32_t D, float *sc)
 {
 #pragma unroll
     for (int r = 0; r < R; r++) sc[r] = 0.f;
-    constexpr int N = Vec<T>::N;
 #pragma unroll 4
-    for (uint32_t d = 0; d < D; d += N) {
-        float k[N];
-        Vec<T>::up(__ldg((const uint4 *)(krow + (size_t)d * sizeof(T))), k);
+    for (uint32_t d = 0; d < D; d += 4) {
+        const float4 k = __ldg((const float4 *)(krow + (size_t)d * 4));
 #pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-            for (int j = 0; j < N; j += 4) {
-                const float4 q = *(const float4 *)&q_s[r][d + j];
-                sc[r] += q.x * k[j] + q.y * k[j + 1] + q.z * k[j + 2] + q.w * k[j + 3];
-            }
+        for (int r = 0; r < R; r++) {
+            const float4 q = *(const float4 *)&q_s[r][d];
+            sc[r] += q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
+        }
     }
 }
 
-template <class T>
 __device__ __forceinline__ void load_q(const RowsDev &q, const RowInfo *ri, float sl2, uint32_t D,
                                        float (*q_s)[kD], int tid, int nt)
 {
@@ -48,13 +42,12 @@ __device__ __forceinline__ void load_q(const RowsDev &q, const RowInfo *ri, floa
         const uint32_t r = e / D, d = e - r * D;
         float x = 0.f;
         if (ri[r].row >= 0)
-            x = to_f(((const T *)(q.p + (long long)ri[r].row * q.row_b +
-                                  (long long)ri[r].head * q.head_b))[d]) * sl2;
+            x = ((const float *)(q.p + (long long)ri[r].row * q.row_b +
+                                 (long long)ri[r].head * q.head_b))[d] * sl2;
         q_s[r][d] = x;
     }
 }
 
-template <class T>
 __global__ void __launch_bounds__(kW * 32)
 attend_simt_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp)
 {
@@ -82,7 +75,7 @@ attend_simt_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp)
             __syncthreads();
             if (threadIdx.x < R) ri[threadIdx.x] = row_info(g, s, at.h, at.rt * R + threadIdx.x);
             __syncthreads();
-            load_q<T>(a.q, ri, a.sl2, D, q_s, threadIdx.x, kW * 32);
+            load_q(a.q, ri, a.sl2, D, q_s, threadIdx.x, kW * 32);
             __syncthreads();
             float m[R], l[R], acc[R][2][4];
 #pragma unroll
@@ -110,7 +103,7 @@ attend_simt_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp)
 #pragma unroll
                 for (int r = 0; r < R; r++) sc[r] = -INFINITY;
                 if (any) {
-                    dots<T>(p.k + off, q_s, D, sc);
+                    dots(p.k + off, q_s, D, sc);
 #pragma unroll
                     for (int r = 0; r < R; r++)
                         if (!(key <= ri[r].hi && key >= ri[r].lo)) sc[r] = -INFINITY;
@@ -145,14 +138,8 @@ attend_simt_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp)
                         for (int j = 0; j < 2; j++) {
                             const uint32_t d = j * 128 + lane * 4;
                             if (d < D) {
-                                const T *vp = (const T *)(p.v + vo) + d;
-                                if (sizeof(T) == 4) {
-                                    const float4 x = __ldg((const float4 *)vp);
-                                    v[j][0] = x.x; v[j][1] = x.y; v[j][2] = x.z; v[j][3] = x.w;
-                                } else {
-#pragma unroll
-                                    for (int q = 0; q < 4; q++) v[j][q] = to_f(vp[q]);
-                                }
+                                const float4 x = __ldg((const float4 *)((const float *)(p.v + vo) + d));
+                                v[j][0] = x.x; v[j][1] = x.y; v[j][2] = x.z; v[j][3] = x.w;
                             }
                         }
                     }
@@ -197,8 +184,8 @@ attend_simt_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp)
                     if (d == 0) { sl[r] = M; sl[R + r] = L; }
                 } else if (ri[r].row >= 0) {
                     const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
-                    ((T *)(a.out.p + (long long)ri[r].row * a.out.row_b +
-                           (long long)ri[r].head * a.out.head_b))[d] = from_f<T>(o * inv);
+                    ((float *)(a.out.p + (long long)ri[r].row * a.out.row_b +
+                               (long long)ri[r].head * a.out.head_b))[d] = o * inv;
                     if (a.lse && d == 0)
                         a.lse[(size_t)ri[r].row * a.Hq + ri[r].head] =
                             L > 0.f ? (Ms + log2f(L)) * 0.69314718055994531f
@@ -217,7 +204,6 @@ attend_simt_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp)
 
 // Masses: a warp takes whole blocks of one (sequence, head), as many as fit 32
 // keys, and walks over all the rows that may attend to them.
-template <class T>
 __global__ void __launch_bounds__(kW * 32)
 mass_simt_kernel(Geo g, PagesDev p, BatchDev b, MassDev a, uint32_t per_warp, uint32_t groups)
 {
@@ -252,14 +238,14 @@ mass_simt_kernel(Geo g, PagesDev p, BatchDev b, MassDev a, uint32_t per_warp, ui
                 lse_s[threadIdx.x] = q.row < 0 ? 0.f : a.lse[(size_t)q.row * a.Hq + q.head];
             }
             __syncthreads();
-            load_q<T>(a.q, ri, a.sl2, p.D, q_s, threadIdx.x, kW * 32);
+            load_q(a.q, ri, a.sl2, p.D, q_s, threadIdx.x, kW * 32);
             __syncthreads();
             bool any = false;
 #pragma unroll
             for (int r = 0; r < R; r++) any |= pg >= 0 && key <= ri[r].hi && key >= ri[r].lo;
             if (!any) continue;
             float sc[R];
-            dots<T>(p.k + off, q_s, p.D, sc);
+            dots(p.k + off, q_s, p.D, sc);
 #pragma unroll
             for (int r = 0; r < R; r++)
                 if (key <= ri[r].hi && key >= ri[r].lo)
@@ -285,35 +271,6 @@ mass_simt_kernel(Geo g, PagesDev p, BatchDev b, MassDev a, uint32_t per_warp, ui
     }
 }
 
-template <class T>
-int attend(const PagesDev &p, const BatchDev &b, const AttendDev &a, const ClassDev &cl,
-           const SplitDev &sp, cudaStream_t s)
-{
-    const Geo g = {kSimtRows, kSimtKeys, a.G, p.H, a.window, cl.min_rows, cl.max_rows, 0};
-    attend_simt_kernel<T><<<sp.ctas, kW * 32, 0, s>>>(g, p, b, a, sp);
-    note_launches(1);
-    OKV_CUDA_TRY(cudaGetLastError());
-    if (sp.ctas > 1) {
-        OKV_CUDA_TRY(launch_after(join_kernel<T, 128>, sp.ctas - 1, 128, 0, s, g, p, b, a, sp, 1u));
-        note_launches(1);
-    }
-    return ORCHKV_OK;
-}
-
-template <class T>
-int mass(const PagesDev &p, const BatchDev &b, const MassDev &a, const ClassDev &cl, cudaStream_t s)
-{
-    const Geo g = {kSimtRows, kSimtKeys, a.G, p.H, a.window, cl.min_rows, cl.max_rows, 0};
-    const uint32_t per_warp = p.bs.d >= 32 ? 1 : 32 / p.bs.d;
-    const uint32_t groups = (b.width + kW * per_warp - 1) / (kW * per_warp);
-    const unsigned long long grid = (unsigned long long)b.n * p.H * groups;
-    if (grid > 0x7FFFFFFFull) return ORCHKV_ERR_INVALID;
-    mass_simt_kernel<T><<<(unsigned)grid, kW * 32, 0, s>>>(g, p, b, a, per_warp, groups);
-    note_launches(1);
-    OKV_CUDA_TRY(cudaGetLastError());
-    return ORCHKV_OK;
-}
-
 }  // namespace
 
 uint32_t attend_simt_ctas(unsigned long long units, unsigned long long keys)
@@ -325,13 +282,29 @@ uint32_t attend_simt_ctas(unsigned long long units, unsigned long long keys)
 int launch_attend_simt(const PagesDev &p, const BatchDev &b, const AttendDev &a,
                        const ClassDev &cl, const SplitDev &sp, cudaStream_t s)
 {
-    return attend<float>(p, b, a, cl, sp, s);
+    const Geo g = {kSimtRows, kSimtKeys, a.G, p.H, a.window, cl.min_rows, cl.max_rows, 0};
+    attend_simt_kernel<<<sp.ctas, kW * 32, 0, s>>>(g, p, b, a, sp);
+    note_launches(1);
+    OKV_CUDA_TRY(cudaGetLastError());
+    if (sp.ctas > 1) {
+        OKV_CUDA_TRY(launch_after(join_kernel<float, 128>, sp.ctas - 1, 128, 0, s, g, p, b, a, sp, 1u));
+        note_launches(1);
+    }
+    return ORCHKV_OK;
 }
 
 int launch_mass_simt(const PagesDev &p, const BatchDev &b, const MassDev &a,
                      const ClassDev &cl, cudaStream_t s)
 {
-    return mass<float>(p, b, a, cl, s);
+    const Geo g = {kSimtRows, kSimtKeys, a.G, p.H, a.window, cl.min_rows, cl.max_rows, 0};
+    const uint32_t per_warp = p.bs.d >= 32 ? 1 : 32 / p.bs.d;
+    const uint32_t groups = (b.width + kW * per_warp - 1) / (kW * per_warp);
+    const unsigned long long grid = (unsigned long long)b.n * p.H * groups;
+    if (grid > 0x7FFFFFFFull) return ORCHKV_ERR_INVALID;
+    mass_simt_kernel<<<(unsigned)grid, kW * 32, 0, s>>>(g, p, b, a, per_warp, groups);
+    note_launches(1);
+    OKV_CUDA_TRY(cudaGetLastError());
+    return ORCHKV_OK;
 }
 
 }  // namespace okv
