@@ -107,7 +107,10 @@ typedef struct orchkv_attend_args {
 /* out[r, h] = sum_t softmax_t(scale * q[r, h] . K[t]) V[t] over the tokens t
  * of r's sequence up to r's own place that lie in a page (and in the
  * window), KV head h / (n_q_heads / n_kv_heads); lse[r, h] = the logarithm of
- * the softmax's denominator.  A row with no such token gets 0 and -infinity.
+ * the softmax's denominator.  A row with no such token gets 0 and -infinity,
+ * and so does one whose scores are all -infinity.  For the second product the
+ * weights are rounded to the pages' type (half a step each; fp16 ones are held
+ * from 2^-25 of a row's largest up, and smaller ones to 2^-36 of it).
  * What lies in places that a row does not attend to does not reach it, be it
  * infinite or NaN; an infinite or NaN value reaches every row that does, as
  * such or as NaN.
@@ -151,7 +154,8 @@ int orchkv_pool_pages(uint32_t n_kv_heads, orchkv_pages_t *out);
  * tokens held.  New tokens get their blocks first: orchkv_append_token_batch
  * (one token, every layer) and orchkv_prefill (one layer) with NULL data
  * allocate and count them, orchkv_paged_append then writes them.
- * Asynchronous on the data plane's stream. */
+ * Runs on the data plane's stream: asynchronous while the requests are those of
+ * the call before, behind a synchronisation of the stream when they are not. */
 int orchkv_slab_table(kv_request_ctx_t *const *ctxs, uint32_t n, uint32_t layer_id, uint32_t n_kv_heads,
                       uint32_t row_len, int32_t *table, int32_t *lens);
 

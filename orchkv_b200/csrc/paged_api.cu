@@ -110,10 +110,10 @@ bool small_call(const orchkv_pages_t *p, const orchkv_batch_t *b, uint64_t G, ui
     return units * ((keys + 63) / 64) <= kSmall * 296;
 }
 
-// What one attend call launches, from what the host knows of it.
 // No sequence is longer than 2^30: a larger window is no window.
 uint32_t window_of(uint32_t w) { return w > (1u << 30) ? 0 : w; }
 
+// What one attend call launches, from what the host knows of it.
 struct AttendPlan {
     SplitDev rows, tile;     // ctas 0: not launched
     ClassDev few, many;

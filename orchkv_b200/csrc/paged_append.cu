@@ -13,8 +13,9 @@
 // token: its threads take a pair's angle each (a double product and a
 // sincospif) and leave it in shared memory for all heads; the norm's weights
 // are multiplied into the rotation's factors once a warp.  6449 tokens of 64/8
-// heads of 128 with norms, bf16: 60.5 us, 4.4 TB/s, 0.67 of the measured copy
-// rate (a warp a token: 78); one token: 2.5 us.
+// heads of 128 with norms, bf16: 60.8 us, 4.3 TB/s, 0.66 of the measured copy
+// rate (a warp a token: 78); one token: 2.5 us.  A lane has two loads in flight,
+// 27 KB an SM with the 27 warps that run; bandwidth x latency asks for 45.
 #include "kernels.h"
 #include "paged.cuh"
 

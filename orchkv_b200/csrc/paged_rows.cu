@@ -15,8 +15,11 @@
 // past the length or in no page are filled with zeros and never read.
 //
 // 32 requests x 1 token over 8192, 28/4 heads of 128, bf16: 96 to 101 us over the
-// boxes measured, 0.81 to 0.85 of the measured copy rate, 6 us of them the join;
-// 61 requests over 1 to 16000 tokens, window 6000: 208 us, 0.91.
+// devices measured, 0.81 to 0.85 of the measured copy rate, 6 us of them the join;
+// 61 requests over 1 to 16000 tokens, window 6000: 208 to 215 us, 0.9.  Chunks
+// that come here reread K and V for every 16 rows: 1024 tokens over 7168, 32/8
+// heads, take 865 us at 128 elements and 24-token pages, 2.60 ms at 256 elements
+// (their products: 78 and 156 us).
 #include <algorithm>
 
 #include "kernels.h"
@@ -396,7 +399,8 @@ attend_rows_kernel(Geo g, PagesDev p, BatchDev b, AttendDev a, SplitDev sp, uint
 // column sums of exp(s - lse) over the 16 rows are three shuffles.  The masses
 // of the run stay in shared memory over the row tiles, so each is written
 // once, in one order of sums.  32 requests x 1 token over 8192, 28/4 heads: 46 to
-// 51 us over the boxes measured, 0.81 to 0.90 of the measured copy rate.
+// 51 us over the devices measured, 0.81 to 0.90 of the measured copy rate; a chunk
+// of 1024 over 7168 of 256 elements, which the tile kernel does not take: 3.09 ms.
 constexpr int kMassStages = 3;
 constexpr uint32_t kMaxRun = 64;                       // blocks of a warp's run
 

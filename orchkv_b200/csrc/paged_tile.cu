@@ -20,15 +20,16 @@
 // neither type nor the fp32 sums mind), which after the first tiles is rare.
 //
 // 4096 new tokens over 28672, 32/8 heads of 128, bf16: 1.77 to 2.01 ms over the
-// boxes measured, 1030 to 1170 TFLOP/s, 0.62 to 0.71 of the measured matrix rate
+// devices measured, 1030 to 1170 TFLOP/s, 0.62 to 0.71 of the measured matrix rate
 // (1654.6).  ncu on 2048 over 6144: tensor pipe 56 % active, special functions
 // 57 %, instruction issue 38 %: what is
 // left is the latency of the chain scores -> maximum -> powers -> weights with
 // two warps a scheduler.  Measured and not kept: a quarter of the powers as
-// polynomials (+3 %), the halves' own S with P over it (2220 us), weights
-// handed over in two parts (+5 %).  A warp whose lanes each issue their page's
-// copy took 4000 clocks a tile for the loads alone; one thread in a loop hides
-// them.
+// polynomials (+3 % at 128 elements; not measured at 64), weights handed over in
+// two parts (+5 %).  A warp whose lanes each issue their page's copy took 4000
+// clocks a tile for the loads alone; one thread in a loop hides them.  An S of
+// its own for each half, with P over it, has been measured with such loads only
+// (2220 us together), not by itself.
 #include <type_traits>
 
 #include "kernels.h"
@@ -603,9 +604,11 @@ int go(const CUtensorMap &km, const CUtensorMap &vm, const PagesDev &p, const Ba
 // list of units as the attention does; pieces of one unit are added by
 // mass_join_kernel in row order.
 //
-// 2048 new tokens over 14336, 32/8 heads of 128, bf16: 272 to 321 us over the
-// boxes measured, 810 to 950 TFLOP/s, 0.49 to 0.57 of the measured matrix rate; 363 us with one group a K tile, 308, 281, 275
-// and 294 us with 1/2, 3/8, 1/4 and none of the powers as polynomials.
+// 2048 new tokens over 14336, 32/8 heads of 128, bf16: 276 to 324 us over the
+// devices and loads measured, 795 to 935 TFLOP/s, 0.48 to 0.57 of the measured
+// matrix rate; of them 5 us keep NaN and infinities in the polynomials.  Before
+// those: 363 us with one group a K tile, 308, 281, 275 and 294 us with 1/2, 3/8,
+// 1/4 and none of the powers as polynomials.
 
 constexpr int kMassThreads = 640;
 constexpr int kMassPoly = 2;                           // of 8 pairs of powers, those on the FMA units
